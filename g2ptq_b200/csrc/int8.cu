@@ -1,0 +1,337 @@
+// 8-bit linears: per-token int8 quantization of activations and the product
+// of int8 codes with a scale per token and per channel.
+//
+//   scale_t = max_c |x_tc| / 127            q_tc = round(x_tc / scale_t)
+//   y_tn    = scale_t * wscale_n * sum_c q_tc w_nc + bias_n
+//
+// The sums are exact in 32-bit integers (|q w| <= 128 * 128, C <= 131071); the
+// only roundings are the conversion of the sum to fp32, the two scalings, the
+// bias and the output type.
+#include "rows.cuh"
+#include "int8.cuh"
+
+namespace g2q {
+namespace i8 {
+
+using rows::of_f;
+using rows::to_f;
+
+// ---------------------------------------------------------------------------
+// quantization of token rows
+// ---------------------------------------------------------------------------
+
+constexpr unsigned kInfBits = 0x7f800000u;
+
+// Sixteen consecutive elements of a row, raw; missing ones (beyond `have`) are zero.
+template <typename S>
+struct Unit {
+  static constexpr int Q = 16 * (int)sizeof(S) / 16;  // 16-byte pieces
+  uint4 raw[Q];
+
+  __device__ __forceinline__ void load(const S* p, int have, bool vec) {
+    if (vec && have >= 16) {
+#pragma unroll
+      for (int i = 0; i < Q; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+      S* e = reinterpret_cast<S*>(raw);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = i < have ? p[i] : of_f<S>(0.f);
+    }
+  }
+  __device__ __forceinline__ float at(int i) const {
+    return to_f<S>(reinterpret_cast<const S*>(raw)[i]);
+  }
+  // the largest magnitude as fp32 bits (ordered as unsigned; infinities and
+  // NaN come out at or above kInfBits)
+  __device__ __forceinline__ unsigned top_bits() const {
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(at(i)) & 0x7fffffffu);
+    return m;
+  }
+};
+
+// round(v / scale), ties to even, of the real quotient: the product with the
+// rounded reciprocal is within 1e-4 of it (|quotient| <= 127), so its rounding
+// is right unless it lands that near a half-integer h; there the sign of the
+// exactly rounded residual v - h * scale decides.
+__device__ __forceinline__ int code_of(float v, float scale, float inv) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
+  const float t = fmaf(v, inv, kMagic);
+  const float n = t - kMagic;
+  const float d = fmaf(v, inv, -n);
+  if (fabsf(d) > 0.4999f) {
+    const float h = n + copysignf(0.5f, d);
+    const float res = fmaf(-h, scale, v);
+    const float lo = h - 0.5f, hi = h + 0.5f;
+    const float even = (static_cast<int>(lo) & 1) ? hi : lo;
+    return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
+  }
+  return static_cast<int>(n);
+}
+
+template <typename S>
+__device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int have, bool vec,
+                                            float scale, float inv, bool finite) {
+  uint32_t w[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      b[i] = finite ? static_cast<uint32_t>(code_of(u.at(4 * g + i), scale, inv)) & 255u : 0u;
+    w[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  }
+  if (vec && have >= 16) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < have) dst[i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
+  }
+}
+
+// G threads per row, UNITS units of 16 elements per thread kept in registers
+// between the maximum and the codes (one read of x); what a longer row has
+// beyond UNITS * G units is read a second time.
+template <typename S, int G, int UNITS>
+__global__ void __launch_bounds__(G > 128 ? G : 128)
+    quantize_kernel(int8_t* __restrict__ codes, long long ldq, float* __restrict__ scale_out,
+                    const S* __restrict__ x, long long ldx, long long T, long long C, bool xvec,
+                    bool qvec) {
+  constexpr int BLOCK = G > 128 ? G : 128;
+  constexpr int PER = BLOCK / G;  // rows per block
+  const int tid = threadIdx.x % G;
+  const long long t = blockIdx.x * (long long)PER + threadIdx.x / G;
+  const bool live = t < T;
+  const S* row = x + (live ? t : 0) * ldx;
+  const long long units = (C + 15) / 16;
+
+  Unit<S> u[UNITS];
+  unsigned top = 0;
+  if (live) {
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k) {
+      const long long i = tid + (long long)k * G;
+      if (i < units) {
+        const long long left = C - 16 * i;
+        u[k].load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < UNITS; ++k)
+      if (tid + (long long)k * G < units) top = max(top, u[k].top_bits());
+    for (long long i = tid + (long long)UNITS * G; i < units; i += G) {
+      const long long left = C - 16 * i;
+      Unit<S> v;
+      v.load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
+      top = max(top, v.top_bits());
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (G > 32) {
+    __shared__ unsigned warp_top[BLOCK / 32];
+    if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
+    __syncthreads();
+    const int w0 = (threadIdx.x / G) * (G / 32);
+#pragma unroll
+    for (int w = 0; w < G / 32; ++w) top = max(top, warp_top[w0 + w]);
+  }
+  if (!live) return;
+  // a value that is not finite makes its whole row NaN: scale NaN, codes zero
+  const bool finite = top < kInfBits;
+  float scale = __fdiv_rn(__uint_as_float(top), 127.f);
+  if (scale < 1.17549435e-38f) scale = 1.f;  // rows of zeros (and of values below normal range)
+  const float inv = __frcp_rn(scale);
+  if (tid == 0) scale_out[t] = finite ? scale : __uint_as_float(0x7fc00000u);
+  int8_t* qrow = codes + t * ldq;
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k) {
+    const long long i = tid + (long long)k * G;
+    if (i < units) {
+      const long long left = C - 16 * i;
+      store_codes<S>(qrow + 16 * i, u[k], left < 16 ? (int)left : 16, qvec, scale, inv, finite);
+    }
+  }
+  for (long long i = tid + (long long)UNITS * G; i < units; i += G) {
+    const long long left = C - 16 * i;
+    Unit<S> v;
+    v.load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
+    store_codes<S>(qrow + 16 * i, v, left < 16 ? (int)left : 16, qvec, scale, inv, finite);
+  }
+}
+
+template <typename S, int G, int UNITS>
+static int launch_quantize(int8_t* codes, long long ldq, float* scale, const S* x, long long ldx,
+                           long long T, long long C, cudaStream_t st) {
+  constexpr int BLOCK = G > 128 ? G : 128;
+  const long long blocks = (T + BLOCK / G - 1) / (BLOCK / G);
+  if (blocks > 0x7fffffffLL) return G2Q_ERR_INVALID_ARG;
+  const bool xvec = rows::aligned(x, 16) && (T <= 1 || (ldx * (long long)sizeof(S)) % 16 == 0);
+  const bool qvec = rows::aligned(codes, 16) && (T <= 1 || ldq % 16 == 0);
+  quantize_kernel<S, G, UNITS><<<(unsigned)blocks, BLOCK, 0, st>>>(codes, ldq, scale, x, ldx, T,
+                                                                   C, xvec, qvec);
+  G2Q_CHECK_LAUNCH();
+  return G2Q_OK;
+}
+
+template <typename S>
+static int quantize_rows(int8_t* codes, long long ldq, float* scale, const void* x, long long ldx,
+                         long long T, long long C, cudaStream_t st) {
+  const S* xs = static_cast<const S*>(x);
+  // One warp per row while a row is at most two units per lane, four warps up
+  // to 8192 columns; sixteen warps for longer rows and where few rows would
+  // leave most SMs idle.
+  if (C > 8192 || T < 2 * 148) return launch_quantize<S, 512, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C > 1024) return launch_quantize<S, 128, 4>(codes, ldq, scale, xs, ldx, T, C, st);
+  return launch_quantize<S, 32, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+}
+
+int quantize_tokens(int8_t* codes, long long ldq, float* scale, const void* x, int dtype,
+                    long long ldx, long long T, long long C, cudaStream_t st) {
+  if (dtype == G2Q_DTYPE_BF16)
+    return quantize_rows<__nv_bfloat16>(codes, ldq, scale, x, ldx, T, C, st);
+  if (dtype == G2Q_DTYPE_F16) return quantize_rows<__half>(codes, ldq, scale, x, ldx, T, C, st);
+  return quantize_rows<float>(codes, ldq, scale, x, ldx, T, C, st);
+}
+
+// ---------------------------------------------------------------------------
+// product on the CUDA cores: operands of any alignment
+// ---------------------------------------------------------------------------
+
+constexpr int ST = 64;   // tile edge (tokens and channels)
+constexpr int SKW = 16;  // 32-bit words of K per step
+
+// The word of codes k .. k+3 of a row, missing ones zero.
+__device__ __forceinline__ int load_word(const int8_t* row, long long k, long long K, bool vec) {
+  if (vec && k + 4 <= K) return *reinterpret_cast<const int*>(row + k);
+  int v = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (k + i < K) v |= (static_cast<int>(row[k + i]) & 255) << (8 * i);
+  return v;
+}
+
+template <typename S>
+__global__ void __launch_bounds__(256) simt_kernel(Product p, bool avec, bool bvec) {
+  __shared__ int as[ST][SKW + 1], bs[ST][SKW + 1];
+  __shared__ Range range;
+  if (threadIdx.x < 32) find_range(p, blockIdx.y, ST, &range);
+  __syncthreads();
+  const Range r = range;
+  if (r.rows <= 0) return;
+  const long long n0 = (long long)blockIdx.x * ST;
+  S* out = static_cast<S*>(p.out);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  int acc[4][4] = {};
+  if (r.group < p.groups) {
+    const int8_t* b = p.b + r.group * p.b_gs;
+    for (long long k0 = 0; k0 < p.K; k0 += 4 * SKW) {
+      for (int i = threadIdx.x; i < ST * SKW; i += 256) {
+        const int row = i / SKW, w = i % SKW;
+        const long long k = k0 + 4 * w;
+        as[row][w] = row < r.rows && k < p.K
+                         ? load_word(p.a + (r.row0 + row) * p.lda, k, p.K, avec) : 0;
+        bs[row][w] = n0 + row < p.N && k < p.K
+                         ? load_word(b + (n0 + row) * p.ldb, k, p.K, bvec) : 0;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < SKW; ++w) {
+        int av[4], bv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) av[i] = as[ty + 16 * i][w];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) bv[j] = bs[tx + 16 * j][w];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(av[i], bv[j], acc[i][j]);
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = ty + 16 * i;
+    if (row >= r.rows) continue;
+    const long long m = r.row0 + row;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long n = n0 + tx + 16 * j;
+      if (n >= p.N) continue;
+      float v = 0.f;  // rows behind the last group
+      if (r.group < p.groups)
+        v = scaled(acc[i][j], p.sa[m], p.sb[r.group * p.N + n], p.bias ? p.bias[n] : 0.f);
+      out[m * p.ldo + n] = of_f<S>(v);
+    }
+  }
+}
+
+static int simt_product(const Product& p, cudaStream_t st) {
+  const long long tiles = range_slots(p, ST);
+  const long long cols = (p.N + ST - 1) / ST;
+  if (tiles > 65535 || cols > 0x7fffffffLL) return G2Q_ERR_UNSUPPORTED;
+  const bool avec = rows::aligned(p.a, 4) && p.lda % 4 == 0;
+  const bool bvec = rows::aligned(p.b, 4) && p.ldb % 4 == 0 && p.b_gs % 4 == 0;
+  const dim3 grid((unsigned)cols, (unsigned)tiles);
+  if (p.out_dtype == G2Q_DTYPE_BF16)
+    simt_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, avec, bvec);
+  else if (p.out_dtype == G2Q_DTYPE_F16)
+    simt_kernel<__half><<<grid, 256, 0, st>>>(p, avec, bvec);
+  else
+    simt_kernel<float><<<grid, 256, 0, st>>>(p, avec, bvec);
+  G2Q_CHECK_LAUNCH();
+  return G2Q_OK;
+}
+
+static int product(const Product& p, cudaStream_t st) { return simt_product(p, st); }
+
+static int check(const Product& p) {
+  if (!rows::elem_bytes(p.out_dtype) || p.M < 0 || p.N <= 0 || p.K <= 0 || p.groups <= 0)
+    return G2Q_ERR_INVALID_ARG;
+  if (p.K > kMaxK || p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.groups > kMaxGroups)
+    return G2Q_ERR_UNSUPPORTED;
+  if (p.M == 0) return G2Q_OK;
+  if (!p.out || !p.a || !p.sa || !p.b || !p.sb || p.lda < p.K || p.ldb < p.K || p.ldo < p.N ||
+      (p.groups > 1 && (!p.offsets || p.b_gs < p.N * p.ldb)))
+    return G2Q_ERR_INVALID_ARG;
+  return G2Q_OK;
+}
+
+}  // namespace i8
+}  // namespace g2q
+
+using namespace g2q;
+
+extern "C" int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, const void* x,
+                                   int dtype, int64_t ldx, int64_t T, int64_t C, void* stream) {
+  if (!rows::elem_bytes(dtype) || T < 0 || C <= 0 || ldx < C || ldq < C) return G2Q_ERR_INVALID_ARG;
+  if (T == 0) return G2Q_OK;
+  if (!codes || !scale || !x) return G2Q_ERR_INVALID_ARG;
+  return i8::quantize_tokens(codes, ldq, scale, x, dtype, ldx, T, C, (cudaStream_t)stream);
+}
+
+extern "C" int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
+                               const float* a_scale, const int8_t* b, int64_t ldb,
+                               const float* b_scale, const float* bias, int64_t M, int64_t N,
+                               int64_t K, int* status, void* stream) {
+  i8::Product p = {out, out_dtype, ldo, a, lda, a_scale, b, ldb, 0, b_scale, bias, nullptr, 1,
+                   M, N, K, status};
+  G2Q_TRY(i8::check(p));
+  if (M == 0) return G2Q_OK;
+  return i8::product(p, (cudaStream_t)stream);
+}
+
+extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t* a,
+                                       int64_t lda, const float* a_scale, const int8_t* b,
+                                       int64_t ldb, int64_t b_gs, const float* b_scale,
+                                       const int32_t* offsets, int64_t G, int64_t M, int64_t N,
+                                       int64_t K, int* status, void* stream) {
+  i8::Product p = {out, out_dtype, ldo, a, lda, a_scale, b, ldb, b_gs, b_scale, nullptr, offsets,
+                   G, M, N, K, status};
+  if (!offsets) return G2Q_ERR_INVALID_ARG;
+  G2Q_TRY(i8::check(p));
+  if (M == 0) return G2Q_OK;
+  return i8::product(p, (cudaStream_t)stream);
+}

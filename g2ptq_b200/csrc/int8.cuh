@@ -1,0 +1,98 @@
+// The 8-bit product's arguments and the mapping of work to row ranges.
+#pragma once
+
+#include "common.cuh"
+
+namespace g2q {
+namespace i8 {
+
+constexpr long long kMaxK = 131071;     // 128 * 128 * K fits an int32 sum
+constexpr long long kMaxGroups = 1024;  // experts
+
+// out[m, n] = sa[m] * sb[g, n] * sum_k a[m, k] * b[g, n, k] + bias[n], with
+// g the group of row m: rows offsets[g] .. offsets[g + 1] - 1 (offsets NULL:
+// one group of all rows).  Rows behind the last group give zeros.
+struct Product {
+  void* out;
+  int out_dtype;
+  long long ldo;
+  const int8_t* a;
+  long long lda;
+  const float* sa;
+  const int8_t* b;
+  long long ldb, b_gs;
+  const float* sb;
+  const float* bias;
+  const int32_t* offsets;
+  long long groups;
+  long long M, N, K;
+  int* status;
+};
+
+// A piece of at most `tile` rows that share one group; group == groups: rows
+// behind the last group; rows <= 0: nothing to do.
+struct Range {
+  long long row0;
+  int rows, group;
+};
+
+// Number of pieces that any offsets can give (the grid's extent).
+static inline long long range_slots(const Product& p, int tile) {
+  const long long full = (p.M + tile - 1) / tile;
+  return p.offsets ? full + (p.groups < p.M ? p.groups : p.M) : full;
+}
+
+// Bounds of group g, made safe against offsets that are not ascending within
+// [0, M]: every piece lies in [0, M].
+__device__ __forceinline__ void group_bounds(const Product& p, long long g, long long* lo,
+                                             long long* hi) {
+  long long a = g == 0 ? 0 : p.offsets[g], b = g < p.groups ? (long long)p.offsets[g + 1] : p.M;
+  a = a < 0 ? 0 : (a > p.M ? p.M : a);
+  b = b < a ? a : (b > p.M ? p.M : b);
+  *lo = a;
+  *hi = b;
+}
+
+// The slot-th piece of `tile` rows, counted through the groups in order (one
+// warp; lane 0 writes *out).
+__device__ __forceinline__ void find_range(const Product& p, long long slot, int tile, Range* out) {
+  const int lane = threadIdx.x & 31;
+  if (!p.offsets) {
+    if (lane == 0) {
+      const long long row0 = slot * tile, left = p.M - row0;
+      *out = Range{row0, (int)(left < tile ? left : tile), 0};
+    }
+    return;
+  }
+  long long before = 0;
+  for (long long g0 = 0; g0 <= p.groups; g0 += 32) {
+    const long long g = g0 + lane;
+    long long lo = 0, hi = 0;
+    if (g <= p.groups) group_bounds(p, g, &lo, &hi);
+    const long long mine = (hi - lo + tile - 1) / tile;
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    const long long first = before + sum - mine;
+    const bool here = slot >= first && slot < first + mine;
+    if (here) {
+      const long long row0 = lo + (slot - first) * tile, left = hi - row0;
+      *out = Range{row0, (int)(left < tile ? left : tile), (int)g};
+    }
+    if (__any_sync(0xffffffffu, here)) return;
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) *out = Range{0, 0, 0};
+}
+
+// The sum scaled: converted to fp32 (rounded once), times the token's and the
+// channel's scale, plus the bias.
+__device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias) {
+  return fmaf(__int2float_rn(acc) * sa, sb, bias);
+}
+
+}  // namespace i8
+}  // namespace g2q

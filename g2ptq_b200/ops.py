@@ -535,3 +535,241 @@ def block_loss_backward(kind, stats, x2, t2, labels, grad_scale=None):
          (t2.stride(0) if rows > 1 else V) if t2 is not None else V, _ptr(gs), rows, V,
          _stream(x2))
     return grad
+
+
+# --------------------------------------------------------------------------
+# 8-bit linears: per-token int8 activations and the scaled integer product
+# --------------------------------------------------------------------------
+
+INT8_MAX_K = 131071  # |a b| <= 128 * 128: longer sums could leave 32 bits
+MAX_EXPERTS = 1024
+
+
+def _call_on(device, name, *args):
+    """``call`` with ``device`` current: a kernel is launched on the current
+    device, which need not be the tensors'."""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
+
+
+def _matrix(name, t):
+    """Row stride of the 2-D ``t`` with unit column stride and rows that do not overlap."""
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} needs unit column stride")
+    if rows <= 1:
+        return max(cols, 1)
+    if t.stride(0) < cols:
+        raise ValueError(f"{name} has overlapping rows")
+    return t.stride(0)
+
+
+def _vector(name, t, n, dtype=torch.float32):
+    if t.shape != (n,) or t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} of shape ({n},), got {t.dtype} of shape "
+                         f"{tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def int8_row_stride(cols):
+    """Row stride of code matrices in memory: rows on 16-byte boundaries, which
+    the tensor-core product needs."""
+    return -(-cols // 16) * 16
+
+
+def quantize_tokens(x):
+    """int8 codes and fp32 scales of every row of ``x [T, C]`` (bf16, fp16 or
+    fp32): ``scale = max |x| / 127``, ``code = round(x / scale)`` with ties to
+    even.  A row whose values are all zero has scale 1; one with an infinity or
+    a NaN has scale NaN and codes 0.  Returns ``(codes [T, C], scale [T])``, the
+    codes' rows ``int8_row_stride(C)`` apart."""
+    dev = _cuda(x)
+    ldx = _matrix("x", x)
+    T, C = x.shape
+    if C == 0:
+        raise ValueError("quantize_tokens needs at least one column")
+    ldq = int8_row_stride(C)
+    codes = torch.empty(T, ldq, dtype=torch.int8, device=dev)[:, :C]
+    scale = torch.empty(T, dtype=torch.float32, device=dev)
+    _call_on(dev, "g2q_quantize_tokens", codes.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(),
+             dtype_code(x.dtype), ldx, T, C, _stream(x))
+    return codes, scale
+
+
+def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
+    """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k] + bias[n]``
+    for int8 ``a [M, K]`` and ``b [N, K]``, fp32 scales and bias; the sums are
+    exact.  Rows 16 bytes aligned (``int8_row_stride``) run on the tensor cores."""
+    dev = _cuda(a, a_scale, b, b_scale, bias)
+    lda, ldb = _matrix("a", a), _matrix("b", b)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise TypeError("int8_matmul takes int8 codes")
+    M, K = a.shape
+    N = b.shape[0]
+    if b.shape[1] != K:
+        raise ValueError(f"a has {K} columns and b {b.shape[1]}")
+    if not 0 < K <= INT8_MAX_K or N == 0:
+        raise ValueError(f"int8_matmul needs 1 to {INT8_MAX_K} columns and at least one channel")
+    _vector("a_scale", a_scale, M)
+    _vector("b_scale", b_scale, N)
+    if bias is not None:
+        _vector("bias", bias, N)
+    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    _call_on(dev, "g2q_int8_matmul", out.data_ptr(), dtype_code(out_dtype), N, a.data_ptr(), lda,
+             a_scale.data_ptr(), b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K,
+             _status(None, dev), _stream(a))
+    return out
+
+
+def _expert_weight(b, b_scale, K):
+    """``(N, ldb, b_gs)`` of the stacked codes ``b [E, N, K]``."""
+    if b.dim() != 3:
+        raise ValueError(f"b must be [experts, channels, columns], got shape {tuple(b.shape)}")
+    E, N, Kb = b.shape
+    if Kb != K:
+        raise ValueError(f"a has {K} columns and b {Kb}")
+    if not 0 < K <= INT8_MAX_K or N == 0 or not 0 < E <= MAX_EXPERTS:
+        raise ValueError(f"needs 1 to {INT8_MAX_K} columns, at least one channel and 1 to "
+                         f"{MAX_EXPERTS} experts")
+    ldb = b.stride(1) if N > 1 else K
+    if (K > 1 and b.stride(2) != 1) or ldb < K or (E > 1 and b.stride(0) < N * ldb):
+        raise ValueError("b needs unit column stride and experts and rows that do not overlap")
+    if b_scale.shape != (E, N) or b_scale.dtype != torch.float32 or not b_scale.is_contiguous():
+        raise ValueError(f"b_scale must be contiguous fp32 of shape ({E}, {N})")
+    return N, ldb, b.stride(0) if E > 1 else N * ldb
+
+
+def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat16):
+    """``int8_matmul`` of rows sorted by expert: rows ``offsets[e]`` to
+    ``offsets[e + 1] - 1`` of ``a [R, K]`` are multiplied with ``b[e]`` of
+    ``b [E, N, K]`` and scaled by ``b_scale [E, N]``.  ``offsets`` is int32
+    ``[E + 1]``, ascending from 0; rows behind ``offsets[E]`` give zeros."""
+    dev = _cuda(a, a_scale, b, b_scale, offsets)
+    lda = _matrix("a", a)
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise TypeError("int8_matmul_grouped takes int8 codes")
+    R, K = a.shape
+    N, ldb, b_gs = _expert_weight(b, b_scale, K)
+    _vector("a_scale", a_scale, R)
+    _vector("offsets", offsets, b.shape[0] + 1, torch.int32)
+    out = torch.empty(R, N, dtype=out_dtype, device=dev)
+    _call_on(dev, "g2q_int8_matmul_grouped", out.data_ptr(), dtype_code(out_dtype), N,
+             a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb, b_gs, b_scale.data_ptr(),
+             offsets.data_ptr(), b.shape[0], R, N, K, _status(None, dev), _stream(a))
+    return out
+
+
+# --------------------------------------------------------------------------
+# Expert routing: sort by expert, rows there and back, gradients
+# --------------------------------------------------------------------------
+
+def route(experts, num_experts):
+    """Sorts the (token, slot) pairs of ``experts [T, k]`` (int32 or int64 ids)
+    by expert, pairs of one expert in their original order.  Returns int32
+    ``(order [T k], position [T, k], offsets [num_experts + 1])``: the pairs
+    ``t k + j`` in expert order, every pair's row there, and each expert's first
+    row.  Pairs whose id is not in ``[0, num_experts)`` come last and have
+    position ``-1 - row``."""
+    dev = _cuda(experts)
+    if experts.dim() != 2 or experts.shape[1] == 0:
+        raise ValueError(f"experts must be [tokens, slots], got shape {tuple(experts.shape)}")
+    if experts.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"experts must be int32 or int64, got {experts.dtype}")
+    if not 0 < num_experts <= MAX_EXPERTS:
+        raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
+    _contig(experts)
+    n = experts.numel()
+    order = torch.empty(n, dtype=torch.int32, device=dev)
+    position = torch.empty(experts.shape, dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    ws_bytes = query("g2q_route_workspace_bytes", n, num_experts)
+    ws = workspace(ws_bytes, dev) if ws_bytes else None
+    _call_on(dev, "g2q_route", order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
+             experts.data_ptr(), int(experts.dtype == torch.int64), n, int(num_experts), _ptr(ws),
+             ws_bytes, _stream(experts))
+    return order, position, offsets
+
+
+def _positions(position):
+    if position.dim() != 2 or position.shape[1] == 0 or position.dtype != torch.int32:
+        raise ValueError("position must be int32 [tokens, slots]")
+    _contig(position)
+    return position.shape
+
+
+def dispatch_rows(x, position):
+    """Rows of ``x [T, C]`` (1-, 2- or 4-byte elements) copied to the rows that
+    ``position [T, k]`` (of ``route``) gives each slot: ``[T k, C]``.  Rows of
+    pairs without an expert are zero."""
+    dev = _cuda(x, position)
+    ldx = _matrix("x", x)
+    T, k = _positions(position)
+    if x.shape[0] != T or x.shape[1] == 0:
+        raise ValueError(f"x must have {T} rows and at least one column")
+    if x.element_size() not in (1, 2, 4):
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    out = torch.empty(T * k, x.shape[1], dtype=x.dtype, device=dev)
+    _call_on(dev, "g2q_dispatch_rows", out.data_ptr(), x.shape[1], x.data_ptr(), ldx,
+             x.element_size(), position.data_ptr(), T, k, x.shape[1], _stream(x))
+    return out
+
+
+def _expert_rows(y, position, weights):
+    T, k = _positions(position)
+    ldy = _matrix("y", y)
+    if y.shape[0] != T * k or y.shape[1] == 0:
+        raise ValueError(f"y must have {T * k} rows and at least one column")
+    if weights is not None:
+        if weights.shape != position.shape:
+            raise ValueError(f"weights must have shape {tuple(position.shape)}")
+        dtype_code(weights.dtype)
+        _contig(weights)
+    return T, k, ldy
+
+
+def combine_rows(y, position, weights=None):
+    """``out[t] = sum_j weights[t, j] * y[position[t, j]]`` over the slots with an
+    expert, added in slot order in fp32 and rounded once to ``y``'s type:
+    ``y [T k, C]``, ``position [T, k]`` of ``route``, ``weights [T, k]`` (None:
+    ones).  A token without any expert gives zeros."""
+    dev = _cuda(y, position, weights)
+    T, k, ldy = _expert_rows(y, position, weights)
+    C = y.shape[1]
+    out = torch.empty(T, C, dtype=y.dtype, device=dev)
+    _call_on(dev, "g2q_combine_rows", out.data_ptr(), C, y.data_ptr(), ldy, dtype_code(y.dtype),
+             position.data_ptr(), _ptr(weights), 0 if weights is None else dtype_code(weights.dtype),
+             T, k, C, _stream(y))
+    return out
+
+
+def combine_rows_backward(grad, y, position, weights, need_y=True, need_weights=True):
+    """Gradients of ``combine_rows`` for the output's gradient ``grad [T, C]``:
+    ``(grad_y [T k, C], grad_weights [T, k])``, None for what is not needed (``y`` is
+    read for the weights' gradient alone).  Rows and weights of pairs without an
+    expert get zero."""
+    y = y if need_weights else None
+    dev = _cuda(grad, y, position, weights)
+    T, k = _positions(position)
+    ldg = _matrix("grad", grad)
+    C = grad.shape[1]
+    if grad.shape[0] != T or C == 0:
+        raise ValueError(f"grad must have {T} rows and at least one column")
+    if weights is None or weights.shape != position.shape:
+        raise ValueError(f"weights must have shape {tuple(position.shape)}")
+    _contig(weights)
+    ldy = C
+    if y is not None:
+        ldy = _matrix("y", y)
+        if y.shape != (T * k, C) or y.dtype != grad.dtype:
+            raise ValueError(f"y must be {grad.dtype} of shape ({T * k}, {C})")
+    gy = torch.empty(T * k, C, dtype=grad.dtype, device=dev) if need_y else None
+    gw = torch.empty(T, k, dtype=weights.dtype, device=dev) if need_weights else None
+    _call_on(dev, "g2q_combine_rows_backward", _ptr(gy), C, _ptr(gw), grad.data_ptr(), ldg,
+             _ptr(y), ldy, dtype_code(grad.dtype), position.data_ptr(), weights.data_ptr(),
+             dtype_code(weights.dtype), T, k, C, _stream(grad))
+    return gy, gw

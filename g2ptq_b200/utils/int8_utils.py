@@ -1,0 +1,104 @@
+"""8-bit linears: what runs a weight that ``fasterquant`` or a ``WeightQuantizer``
+quantized to int8 codes with one scale per channel.
+
+Activations are quantized per token as they arrive (the reference's per-token
+symmetric ``ActQuantizer``, utils/quant_utils.py:167-338, which only emulates it
+in the model's type); the codes are multiplied as integers and the sums scaled
+per token and per channel.  Inference only: nothing here records gradients.
+"""
+
+import torch
+
+from .. import ops
+
+
+def _int8_rows(codes):
+    """``codes`` in memory with rows on 16-byte boundaries."""
+    *lead, cols = codes.shape
+    out = torch.zeros(*lead, ops.int8_row_stride(cols), dtype=torch.int8, device=codes.device)
+    out = out[..., :cols]
+    out.copy_(codes)
+    return out
+
+
+def int8_linear(x, codes, scale, bias=None):
+    """``x @ (scale[:, None] * codes).T + bias`` with ``x [..., K]`` quantized per
+    token: int8 ``codes [N, K]``, fp32 ``scale [N]`` and ``bias [N]``.  The result
+    has ``x``'s type."""
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x2.shape[1] > 1 and x2.stride(1) != 1:
+        x2 = x2.contiguous()
+    q, s = ops.quantize_tokens(x2)
+    y = ops.int8_matmul(q, s, codes, scale, bias, out_dtype=x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
+
+
+def int8_experts(x, codes, scale, offsets):
+    """``int8_linear`` of rows sorted by expert (``moe_utils.dispatch``): rows
+    ``offsets[e]`` to ``offsets[e + 1] - 1`` of ``x [R, K]`` through expert
+    ``e``'s ``codes [E, N, K]`` and ``scale [E, N]``.  Rows behind the last
+    expert's give zeros."""
+    if x.dim() == 2 and x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    q, s = ops.quantize_tokens(x)
+    return ops.int8_matmul_grouped(q, s, codes, scale, offsets, out_dtype=x.dtype)
+
+
+def weight_codes(weight, quantizer):
+    """int8 codes ``[N, K]`` and fp32 scales ``[N]`` of ``weight`` on the grid of a
+    ready ``WeightQuantizer``: symmetric, one scale per channel."""
+    if not quantizer.ready() or not quantizer.sym or quantizer.weight_groupsize > 0:
+        raise ValueError("8-bit linears need a ready symmetric quantizer with one scale per "
+                         "channel (no groups)")
+    if quantizer.bits > 8:
+        raise ValueError(f"codes of {quantizer.bits} bits do not fit int8")
+    if quantizer.scale.numel() not in (1, weight.shape[0]):
+        raise ValueError(f"the quantizer has {quantizer.scale.numel()} scales for "
+                         f"{weight.shape[0]} channels (of a layer-batched object take each "
+                         "layer's rows with merge_group_quantizers)")
+    _, q, scale = quantizer.fake_quantize(weight)
+    scale = scale.reshape(-1).float()
+    if scale.numel() == 1:
+        scale = scale.expand(weight.shape[0])
+    return q.to(torch.int8), scale.contiguous()
+
+
+class Int8Linear(torch.nn.Module):
+    """A linear that holds int8 codes and channel scales."""
+
+    def __init__(self, codes, scale, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = codes.shape
+        self.register_buffer("codes", _int8_rows(codes))
+        self.register_buffer("scale", scale.detach().reshape(-1).float().contiguous())
+        self.register_buffer("bias", None if bias is None else bias.detach().float().contiguous())
+
+    @classmethod
+    def from_linear(cls, linear, quantizer):
+        """The codes of ``linear.weight`` on ``quantizer``'s grid: after
+        ``fasterquant`` with that quantizer (``obj.quantizer[0]`` for
+        ``groupsize`` -1), the codes it chose."""
+        codes, scale = weight_codes(linear.weight.data, quantizer)
+        return cls(codes, scale, linear.bias)
+
+    @torch.no_grad()
+    def forward(self, x):
+        return int8_linear(x, self.codes, self.scale, self.bias)
+
+
+class Int8Experts(torch.nn.Module):
+    """The same projection of every expert of an MoE layer, stacked."""
+
+    def __init__(self, codes, scale):
+        super().__init__()
+        self.register_buffer("codes", _int8_rows(codes))
+        self.register_buffer("scale", scale.detach().float().contiguous())
+
+    @classmethod
+    def from_linears(cls, linears, quantizers):
+        pairs = [weight_codes(lin.weight.data, q) for lin, q in zip(linears, quantizers)]
+        return cls(torch.stack([c for c, _ in pairs]), torch.stack([s for _, s in pairs]))
+
+    @torch.no_grad()
+    def forward(self, rows, offsets):
+        return int8_experts(rows, self.codes, self.scale, offsets)

@@ -450,6 +450,76 @@ int g2q_block_loss_backward(int kind, void* grad, int64_t ldg, const float* row_
                             int64_t ldx, int64_t ldt, const float* grad_scale, int64_t rows,
                             int64_t V, void* stream);
 
+/* ---- 8-bit linears ----
+ * The product that runs a weight quantized to int8 codes with one scale per
+ * channel, with activations quantized per token.  Replaces the per-token
+ * activation quantizer and the linear behind it (utils/quant_utils.py:167-338,
+ * which quantize, dequantize and multiply in the model's type). */
+
+/* codes[t][c] = round(x[t][c] / scale[t]), ties to even, with scale[t] =
+ * fp32(max_c |x[t][c]| / 127): x [T, C] of type dtype (row stride ldx), codes
+ * [T, C] (row stride ldq), scale [T].  The quotient is rounded as the real
+ * number it is.  Rows whose scale would be below the smallest normal fp32
+ * number (rows of zeros) get scale 1; rows with an infinity or a NaN get scale
+ * NaN and codes 0. */
+int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, const void* x, int dtype,
+                        int64_t ldx, int64_t T, int64_t C, void* stream);
+
+/* out[m][n] = a_scale[m] * b_scale[n] * sum_k a[m][k] * b[n][k] + bias[n]:
+ * int8 a [M, K] and b [N, K] (row strides lda, ldb), fp32 a_scale [M], b_scale
+ * [N] and bias [N] (may be NULL), out [M, N] of type out_dtype (row stride
+ * ldo).  The sums are exact 32-bit integers: K above 131071 is unsupported. */
+int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
+                    const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
+                    const float* bias, int64_t M, int64_t N, int64_t K, int* status,
+                    void* stream);
+
+/* The same for rows sorted into G groups: rows offsets[g] .. offsets[g+1] - 1
+ * (device int32 [G + 1], ascending from 0, at most M) use b + g * b_gs and
+ * b_scale + g * N.  Rows behind offsets[G] give zeros.  G above 1024 is
+ * unsupported. */
+int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
+                            const float* a_scale, const int8_t* b, int64_t ldb, int64_t b_gs,
+                            const float* b_scale, const int32_t* offsets, int64_t G, int64_t M,
+                            int64_t N, int64_t K, int* status, void* stream);
+
+/* ---- expert routing ----
+ * Replaces the per-expert index, gather and index_add of the routed expert
+ * forward (utils/models/mixins.py:233-259). */
+
+/* Stable counting sort of n = T * k (token, slot) pairs by expert id (ids
+ * [T, k] contiguous, int64 when ids_wide, else int32): order[r] = the pair in
+ * row r, position[pair] = its row, offsets[e] = the first row of expert e
+ * (offsets[E] = the number of pairs with an expert).  Pairs whose id is not in
+ * [0, E) come last; their position is -1 - row.  E above 1024 is unsupported.
+ * `workspace`: g2q_route_workspace_bytes(n, E) bytes (0 for short inputs). */
+int g2q_route(int32_t* order, int32_t* position, int32_t* offsets, const void* ids, int ids_wide,
+              int64_t n, int64_t E, void* workspace, size_t workspace_bytes, void* stream);
+size_t g2q_route_workspace_bytes(int64_t n, int64_t E);
+
+/* out[r] = x[t] for r = position[t][j] >= 0, zeros for row -1 - position[t][j]
+ * of a pair without an expert: x [T, C], out [T * k, C], strides in elements of
+ * elem_size (1, 2 or 4) bytes.  Positions outside of [-T k, T k) are skipped. */
+int g2q_dispatch_rows(void* out, int64_t ldo, const void* x, int64_t ldx, int elem_size,
+                      const int32_t* position, int64_t T, int64_t k, int64_t C, void* stream);
+
+/* out[t] = sum_j weights[t][j] * y[position[t][j]] over the slots whose
+ * position is not negative, in slot order in fp32, rounded once: y [T * k, C]
+ * and out [T, C] of type dtype; weights [T, k] of type w_dtype, NULL = ones
+ * (with which it is also the gradient of g2q_dispatch_rows). */
+int g2q_combine_rows(void* out, int64_t ldo, const void* y, int64_t ldy, int dtype,
+                     const int32_t* position, const void* weights, int w_dtype, int64_t T,
+                     int64_t k, int64_t C, void* stream);
+
+/* Gradients of g2q_combine_rows for grad [T, C] (type dtype): grad_y [T k, C]
+ * row position[t][j] = weights[t][j] * grad[t]; grad_w[t][j] (type w_dtype) =
+ * <grad[t], y[position[t][j]]> in fp32.  Pairs without an expert get zeros.
+ * Either of grad_y, grad_w may be NULL. */
+int g2q_combine_rows_backward(void* grad_y, int64_t ldgy, void* grad_w, const void* grad,
+                              int64_t ldg, const void* y, int64_t ldy, int dtype,
+                              const int32_t* position, const void* weights, int w_dtype,
+                              int64_t T, int64_t k, int64_t C, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
