@@ -92,7 +92,8 @@ SIGNATURES = {
     "g2q_block_loss_forward": [I32, P, P, P, P, P, I32, I64, I64, I64, I64, P],
     "g2q_block_loss_backward": [I32, P, I64, P, P, P, P, I32, I64, I64, P, I64, I64, P],
     "g2q_quantize_tokens": [P, I64, P, P, I32, I64, I64, I64, P],
-    "g2q_int8_matmul": [P, I32, I64, P, I64, P, P, I64, P, P, I64, I64, I64, P, P],
+    "g2q_int8_matmul": [P, I32, I64, P, I64, P, P, I64, P, P, I64, I64, I64, P, SZ, P, P],
+    "g2q_int8_matmul_workspace_bytes": [I64, I64, I64],
     "g2q_int8_matmul_grouped": [P, I32, I64, P, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P,
                                 P],
     "g2q_route": [P, P, P, P, I32, I64, I64, P, SZ, P],
@@ -111,6 +112,7 @@ _RESTYPES = {
     "g2q_compensate_workspace_bytes": SZ,
     "g2q_gemm_tc_workspace_bytes": SZ,
     "g2q_gram_static_scratch_bytes": SZ,
+    "g2q_int8_matmul_workspace_bytes": SZ,
     "g2q_route_workspace_bytes": SZ,
 }
 

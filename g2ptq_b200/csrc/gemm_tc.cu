@@ -42,6 +42,7 @@
 #include <cuda_fp16.h>
 
 #include "gemm_simt.cuh"
+#include "tc_ptx.cuh"
 
 namespace g2q {
 namespace tc {
@@ -49,8 +50,6 @@ namespace tc {
 constexpr int BM = 128, BN = 128, BK = 64;
 constexpr int CHUNK_BYTES = 64 * BK * 2;     // one 64 (MN) x 64 (K) bf16 box
 constexpr int TILE_BYTES = 2 * CHUNK_BYTES;  // one 128 x 64 operand tile
-constexpr long long kWaitCycles = 4000000000LL;   // default bound of one pipeline wait
-constexpr long long kDrainCycles = 2000000000LL;  // bound of a wind-down wait after an abort
 
 struct Params {
   float* D;
@@ -76,67 +75,6 @@ struct Params {
   int* status;     // receives G2Q_ERR_TIMEOUT when a wait gives up (may be null)
   long long wait_cycles;  // bound of every pipeline wait (set by the launchers)
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t a, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t a, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes)
-               : "memory");
-}
-
-__device__ __forceinline__ bool mbar_test(uint32_t a, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(done)
-      : "r"(a), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-// Pipeline wait: gives up when another warp of the CTA has given up
-// (abort_flag) or after `limit` cycles, which sets the flag and records
-// G2Q_ERR_TIMEOUT.
-__device__ __forceinline__ bool mbar_wait(uint32_t a, uint32_t parity, volatile int* abort_flag,
-                                          int* status, long long limit) {
-  const long long t0 = clock64();
-  while (true) {
-    if (mbar_test(a, parity)) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > limit) {
-      *abort_flag = 1;
-      record_error(status, G2Q_ERR_TIMEOUT);
-      return false;
-    }
-  }
-}
-
-// Wind-down wait after an abort: the phase completes once asynchronous work
-// this thread already issued (loads, MMAs) has finished; bounded by
-// kDrainCycles, and it ignores the abort flag.
-__device__ __forceinline__ bool mbar_drain(uint32_t a, uint32_t parity) {
-  const long long t0 = clock64();
-  while (!mbar_test(a, parity))
-    if (clock64() - t0 > kDrainCycles) return false;
-  return true;
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                            uint32_t mbar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
-      : "memory");
-}
 
 // D[z][y .. y+31][x .. x+31] += the 32 x 32 fp32 box at smem (128-byte swizzled
 // rows), performed by the TMA unit in L2: the SM never reads D.
@@ -203,37 +141,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t a, uint64_t 
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-
-__device__ __forceinline__ void umma_commit(uint32_t mbar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   mbar)
-               : "memory");
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t a) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
-}
-
-__device__ __forceinline__ void fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // SMALL: short-K variant (K <= 4 blocks, no promotion needed): one accumulator,
@@ -706,40 +613,6 @@ struct PairCfg {
   static constexpr int PROMOTE_KB = (NA == 1 ? 8 : 4) * BK / BKP;
 };
 
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-
-// shared::cluster address of the variable at shared::cta address a in CTA rank
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t a, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(rank));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
-               "barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
-                                                 uint32_t mbar_cluster) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar_cluster)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
-  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y)
-               : "memory");
-}
-
 __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t a, uint64_t b,
                                                uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -747,26 +620,6 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t tmem_d, uint64_t a, uint
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
       "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
-}
-
-// arrive on the barrier at shared::cta offset mbar in both CTAs of the pair
-// once every MMA issued so far by this thread has completed
-__device__ __forceinline__ void umma_commit_pair(uint32_t mbar) {
-  const uint16_t mask = 0x3;
-  asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%0], %1;" ::"r"(mbar),
-      "h"(mask)
-      : "memory");
-}
-
-// Arrive on a barrier of either CTA of the pair.  The drained-accumulator
-// barrier carries no memory data: the TMEM reads before it are ordered against
-// the MMAs after it by the tcgen05 fences on both sides, so the default
-// (CTA-scope) semantics suffice; a cluster-scope release here costs a memory
-// barrier per epilogue warp and drain.
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t mbar_cluster) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(mbar_cluster) : "memory");
 }
 
 __host__ __device__ constexpr uint32_t idesc_bf16_mn_m256(int n) {
@@ -988,19 +841,6 @@ __global__ void __launch_bounds__(PairCfg<NA, BKP>::THREADS, 1)
 // host side
 // ---------------------------------------------------------------------------
 
-static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  if (!fn) {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
-            cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  }
-  return fn;
-}
-
 // 2-D bf16 tensor [outer, inner] with row stride ld (elements), 64 x 64 boxes.
 static bool make_map(CUtensorMap* m, const void* base, long long inner, long long outer,
                      long long ld, bool f16 = false, int box_k = BK) {
@@ -1046,6 +886,7 @@ static bool make_map_out(CUtensorMap* m, float* D, long long N, long long M, lon
 // Bound of every pipeline wait of the tensor-core kernels, in SM clock cycles
 // (g2q_set_wait_limit); read at each launch.
 static volatile long long g_wait_cycles = kWaitCycles;
+long long wait_cycles() { return g_wait_cycles; }
 
 template <int NA, int NB, bool SMALL, bool WIDE = false>
 static int launch(const Maps& m, const Params& p, long long batch, cudaStream_t st) {

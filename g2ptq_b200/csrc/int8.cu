@@ -285,7 +285,9 @@ static int simt_product(const Product& p, cudaStream_t st) {
   return G2Q_OK;
 }
 
-static int product(const Product& p, cudaStream_t st) { return simt_product(p, st); }
+static int product(const Product& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  return tc_takes(p) ? tc_product(p, workspace, workspace_bytes, st) : simt_product(p, st);
+}
 
 static int check(const Product& p) {
   if (!rows::elem_bytes(p.out_dtype) || p.M < 0 || p.N <= 0 || p.K <= 0 || p.groups <= 0)
@@ -312,15 +314,27 @@ extern "C" int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, con
   return i8::quantize_tokens(codes, ldq, scale, x, dtype, ldx, T, C, (cudaStream_t)stream);
 }
 
+extern "C" size_t g2q_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || K > i8::kMaxK || M > 0x7fffffffLL || N > 0x7fffffffLL) return 0;
+  i8::Product p = {};
+  p.lda = p.ldb = (K + 15) / 16 * 16;
+  p.groups = 1;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  return i8::tc_workspace_bytes(p);
+}
+
 extern "C" int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
                                const float* a_scale, const int8_t* b, int64_t ldb,
                                const float* b_scale, const float* bias, int64_t M, int64_t N,
-                               int64_t K, int* status, void* stream) {
+                               int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                               void* stream) {
   i8::Product p = {out, out_dtype, ldo, a, lda, a_scale, b, ldb, 0, b_scale, bias, nullptr, 1,
                    M, N, K, status};
   G2Q_TRY(i8::check(p));
   if (M == 0) return G2Q_OK;
-  return i8::product(p, (cudaStream_t)stream);
+  return i8::product(p, workspace, workspace_bytes, (cudaStream_t)stream);
 }
 
 extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t* a,
@@ -333,5 +347,5 @@ extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, co
   if (!offsets) return G2Q_ERR_INVALID_ARG;
   G2Q_TRY(i8::check(p));
   if (M == 0) return G2Q_OK;
-  return i8::product(p, (cudaStream_t)stream);
+  return i8::product(p, nullptr, 0, (cudaStream_t)stream);
 }

@@ -1,0 +1,526 @@
+// The 8-bit product on the tensor cores (tcgen05 kind::i8, 32-bit integer sums
+// in TMEM).
+//
+// A cluster of two CTAs computes tiles of 256 channels x up to 256 tokens
+// (cta_group::2, M = 256 channels, N = the piece's tokens rounded up to 64):
+// CTA r of the pair loads channels ch0 + 128 r .. + 127 of the weight and its
+// half of the tokens, the leader issues the MMAs, and each CTA's TMEM receives
+// its own 128 channels x all tokens.  The channels are the M side because the
+// rows of a group end anywhere: a short piece then costs a smaller N, where
+// tokens on the M side would always pay for 256.  The integer sums are exact,
+// so one accumulator runs over the whole K; the two 256-column TMEM buffers let
+// the epilogue of one tile overlap the next tile's products.
+//
+// The grid is persistent (one cluster per SM pair); each cluster walks the
+// tiles in steps of the cluster count, in groups of eight row pieces so that
+// weights and tokens meet in L2.  Where there are fewer tiles than clusters, K
+// is cut into `splits` ranges whose 32-bit sums go to a workspace and are added
+// and scaled by a second kernel (integers: the order does not matter).
+//
+// Warp roles per CTA (320 threads): warp 0 TMA producer, warp 1 TMEM owner and
+// (leader) MMA issuer, warps 2-9 epilogue.  Every wait is bounded as in the
+// Gram kernels; on expiry G2Q_ERR_TIMEOUT goes to the status word and the CTAs
+// wind down.
+#include "int8.cuh"
+#include "rows.cuh"
+#include "tc_ptx.cuh"
+
+namespace g2q {
+namespace i8 {
+
+using namespace g2q::tc;
+using rows::of_f;
+
+constexpr int CH = 256;              // channels per tile (128 per CTA)
+constexpr int TOK = 256;             // most tokens per tile
+constexpr int KB = 128;              // bytes of K per operand chunk (one swizzled row)
+constexpr int KC = 2;                // chunks per pipeline stage
+constexpr int OP_BYTES = 128 * KB;   // one operand's chunk in one CTA
+constexpr int STAGE_BYTES = KC * 2 * OP_BYTES;
+constexpr int STAGES = 3;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int RASTER = 8;            // row pieces walked together
+
+struct TcArgs {
+  Product p;
+  int ch_tiles, nk;              // channel tiles; chunks of K
+  int splits, per_split;         // K ranges and chunks in each
+  int32_t* part;                 // [splits][M][N] when splits > 1
+  long long wait_cycles;
+};
+
+// What one cluster works on
+struct Tile {
+  long long row0;
+  int rows, group, ch0, k0, k1;  // k: chunks
+  int split;
+};
+
+// In shared memory: the first piece of each group and the groups' bounds, so
+// that every role finds its tile by a binary search.
+struct Table {
+  int32_t* first;  // [groups + 2]
+  int32_t* lo;     // [groups + 1]
+  int32_t* hi;
+};
+
+__device__ __forceinline__ void build_table(const Product& p, const Table& t) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+    const int g = g0 + lane;
+    long long lo = 0, hi = 0;
+    if (g <= p.groups) {
+      if (p.offsets) {
+        group_bounds(p, g, &lo, &hi);
+      } else {
+        lo = g == 0 ? 0 : p.M;
+        hi = p.M;
+      }
+      t.lo[g] = (int)lo;
+      t.hi[g] = (int)hi;
+    }
+    const int mine = (int)((hi - lo + TOK - 1) / TOK);
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (g <= p.groups) t.first[g] = before + sum - mine;
+    before += __shfl_sync(0xffffffffu, sum, 31);
+  }
+  if (lane == 0) t.first[p.groups + 1] = before;
+}
+
+__device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, long long w) {
+  Tile r;
+  r.split = (int)(w % a.splits);
+  w /= a.splits;
+  const int pieces = t.first[a.p.groups + 1];
+  const int r0 = (int)(w / ((long long)RASTER * a.ch_tiles)) * RASTER;
+  const int gsz = pieces - r0 < RASTER ? pieces - r0 : RASTER;
+  const int rem = (int)(w - (long long)r0 * a.ch_tiles);
+  const int piece = r0 + rem % gsz;
+  r.ch0 = rem / gsz * CH;
+  int lo = 0, hi = (int)a.p.groups;  // the last group with first <= piece
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (t.first[mid] <= piece) lo = mid;
+    else hi = mid - 1;
+  }
+  r.group = lo;
+  r.row0 = t.lo[lo] + (long long)(piece - t.first[lo]) * TOK;
+  const long long left = t.hi[lo] - r.row0;
+  r.rows = (int)(left < TOK ? left : TOK);
+  r.k0 = r.split * a.per_split;
+  r.k1 = r.k0 + a.per_split < a.nk ? r.k0 + a.per_split : a.nk;
+  return r;
+}
+
+__device__ __forceinline__ int mma_n(int rows) { return (rows + 63) / 64 * 64; }
+
+// Shared-memory descriptor of a K-major operand: rows of 128 swizzled bytes,
+// groups of eight rows 1 KB apart.
+__device__ __forceinline__ uint64_t desc_k_sw128(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// kind::i8 instruction descriptor: signed x signed -> s32, both K-major, M = 256
+__device__ __forceinline__ uint32_t idesc_i8_m256(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(CH >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t a, uint64_t b,
+                                             uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                                 int z, uint32_t mbar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(mbar_cluster)
+      : "memory");
+}
+
+template <typename S>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  S v[2] = {of_f<S>(a), of_f<S>(b)};
+  return *reinterpret_cast<uint32_t*>(v);
+}
+
+// 32 columns (tokens) of this lane's channel into out; the warp's 32 lanes are
+// 32 neighbouring channels.  16-bit outputs go two channels at a time: lane
+// pairs exchange so that the even lane holds both channels of the even token,
+// the odd lane both of the odd token.
+template <typename S>
+__device__ __forceinline__ void store_block(S* out, long long ldo, const float* sa, int rows,
+                                            const uint32_t (&r)[32], float sb, float bias,
+                                            long long n, long long N, bool paired, bool zero) {
+  const int lane = threadIdx.x & 31;
+  if (sizeof(S) == 2 && paired) {
+    const int odd = lane & 1;
+    S* dst = out + odd * ldo + (n - odd);
+    const bool in = n - odd + 1 < N;
+#pragma unroll
+    for (int c = 0; c < 32; c += 2) {
+      float v0 = zero ? 0.f : scaled((int)r[c], sa[c], sb, bias);
+      float v1 = zero ? 0.f : scaled((int)r[c + 1], sa[c + 1], sb, bias);
+      const float other = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
+      const uint32_t w = odd ? pack2<S>(other, v1) : pack2<S>(v0, other);
+      if (in && c + odd < rows) *reinterpret_cast<uint32_t*>(dst + c * ldo) = w;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 32; ++c)
+      if (n < N && c < rows)
+        out[c * ldo + n] = of_f<S>(zero ? 0.f : scaled((int)r[c], sa[c], sb, bias));
+  }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(THREADS, 1)
+    tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mt128,
+              const __grid_constant__ CUtensorMap mt32, const TcArgs a) {
+  const Product& p = a.p;
+  const uint32_t rank = cluster_ctarank();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  // bars[0..S): full (leader's used), [S..2S): empty, [2S..2S+2): accumulator full,
+  // [2S+2..2S+4): accumulator drained (leader's used), [2S+4]: MMA completion after an abort
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  float* sa_s = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 128);  // [2][TOK]
+  Table table;
+  table.first = reinterpret_cast<int32_t*>(sa_s + 2 * TOK);
+  table.lo = table.first + p.groups + 2;
+  table.hi = table.lo + p.groups + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+  const uint32_t accf0 = smem_u32(bars + 2 * STAGES);
+  const uint32_t acce0 = smem_u32(bars + 2 * STAGES + 2);
+  const uint32_t drain0 = smem_u32(bars + 2 * STAGES + 4);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(full0 + 8 * s, 1);
+        mbar_init(empty0 + 8 * s, 1);
+      }
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(accf0 + 8 * b, 1);
+        mbar_init(acce0 + 8 * b, 2 * EPI_WARPS);
+      }
+      mbar_init(drain0, 1);
+      *abort_flag = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+  } else if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_holder)),
+                 "r"(2 * TOK)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else if (warp == 2) {
+    build_table(p, table);
+  }
+  fence_before();
+  __syncthreads();
+  cluster_sync();  // barriers of both CTAs initialised, TMEM allocated in both
+  fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const long long total = (long long)table.first[p.groups + 1] * a.ch_tiles * a.splits;
+  const long long step = gridDim.x >> 1;
+
+  int issued = 0;  // stages whose loads this CTA's producer issued
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint32_t full_lead = mapa_shared(full0, 0);
+      bool ok = true;
+      for (long long w = blockIdx.x >> 1; ok && w < total; w += step) {
+        const Tile t = decode(a, table, w);
+        if (t.group == p.groups) continue;
+        const int half = mma_n(t.rows) / 2;
+        const int y = (int)t.row0 + (int)rank * half;
+        const int ych = t.ch0 + 128 * (int)rank;
+        for (int k = t.k0; k < t.k1; k += KC) {
+          const int s = issued % STAGES;
+          const uint32_t ph = (issued / STAGES) & 1;
+          ok = mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, a.wait_cycles);
+          if (!ok) break;
+          ++issued;
+          const int nc = t.k1 - k < KC ? t.k1 - k : KC;
+          // the leader's full[s] expects the bytes of both CTAs
+          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * nc * (OP_BYTES + half * KB));
+          const uint32_t fb = full_lead + 8 * s;
+          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+          for (int c = 0; c < nc; ++c) {
+            const int x = (k + c) * KB;
+            tma_load_3d_pair(st + c * OP_BYTES, &mw, x, ych, t.group, fb);
+            const uint32_t sb = st + (KC + c) * OP_BYTES;
+            if (half == 128) {
+              tma_load_2d_pair(sb, &mt128, x, y, fb);
+            } else {
+              for (int i = 0; i < half; i += 32) tma_load_2d_pair(sb + i * KB, &mt32, x, y + i, fb);
+            }
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int it = 0, tc = 0;
+      bool ok = true;
+      for (long long w = blockIdx.x >> 1; ok && w < total; w += step) {
+        const Tile t = decode(a, table, w);
+        if (t.group == p.groups) continue;
+        const int buf = tc & 1;
+        const uint32_t use_ph = (uint32_t)((tc >> 1) & 1);
+        ++tc;
+        ok = mbar_wait(acce0 + 8 * buf, use_ph ^ 1, abort_flag, p.status, a.wait_cycles);
+        if (!ok) break;
+        fence_after();
+        const uint32_t acc = tmem + (uint32_t)(buf * TOK);
+        const uint32_t idesc = idesc_i8_m256(mma_n(t.rows));
+        for (int k = t.k0; k < t.k1; k += KC) {
+          const int s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          ok = mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, a.wait_cycles);
+          if (!ok) break;
+          ++it;
+          fence_after();
+          const int nc = t.k1 - k < KC ? t.k1 - k : KC;
+          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+          for (int c = 0; c < nc; ++c) {
+            const uint64_t da = desc_k_sw128(st + c * OP_BYTES);
+            const uint64_t db = desc_k_sw128(st + (KC + c) * OP_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < KB / 32; ++kk)  // 32 bytes of K per MMA
+              umma_i8_pair(acc, da + 2 * kk, db + 2 * kk, idesc,
+                           k > t.k0 || c > 0 || kk > 0 ? 1u : 0u);
+          }
+          umma_commit_pair(empty0 + 8 * s);
+        }
+        if (ok) umma_commit_pair(accf0 + 8 * buf);
+      }
+    }
+  } else {
+    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (channels) of this CTA; the two
+    // warps of a quadrant take alternate blocks of 32 tokens
+    const int q = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
+    const uint32_t acce_lead = mapa_shared(acce0, 0);
+    S* out = static_cast<S*>(p.out);
+    const bool paired = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && p.ldo % 2 == 0 &&
+                        p.N % 2 == 0;
+    int tc = 0, turn = 0;
+    bool ok = true;
+    for (long long w = blockIdx.x >> 1; w < total; w += step, ++turn) {
+      const Tile t = decode(a, table, w);
+      const bool zero = t.group == p.groups;
+      const long long n = t.ch0 + 128 * (int)rank + q * 32 + lane;
+      float* sa = sa_s + (turn & 1) * TOK;
+      sa[et] = et < t.rows ? p.sa[t.row0 + et] : 0.f;
+      const float sb = !zero && n < p.N ? p.sb[(long long)t.group * p.N + n] : 0.f;
+      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+      const int buf = tc & 1;
+      if (!zero) {
+        const uint32_t use_ph = (uint32_t)((tc >> 1) & 1);
+        ++tc;
+        if (ok) ok = mbar_wait(accf0 + 8 * buf, use_ph, abort_flag, p.status, a.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        fence_after();
+      }
+      const uint32_t base = tmem + (uint32_t)(buf * TOK) + ((uint32_t)(q * 32) << 16);
+      for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
+        uint32_t r[32];
+        if (!zero) tmem_ld32(base + (uint32_t)c0, r);
+        if (!ok) continue;
+        if (a.splits > 1) {
+          int32_t* dst = a.part + ((long long)t.split * p.M + t.row0 + c0) * p.N + n;
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (n < p.N && c0 + c < t.rows) dst[c * p.N] = (int)r[c];
+        } else {
+          store_block<S>(out + (t.row0 + c0) * p.ldo, p.ldo, sa + c0, t.rows - c0, r, sb, bias, n,
+                         p.N, paired, zero);
+        }
+      }
+      if (!zero) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(acce_lead + 8 * buf);
+      }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    // a wait gave up: the leader lets the loads into the stages it armed land and
+    // its MMAs finish; the peer, whose loads complete no barrier of its own,
+    // allows them a fixed settling time
+    if (warp == 0 && lane == 0) {
+      if (rank == 0) {
+        for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+          mbar_drain(full0 + 8 * (i % STAGES), (i / STAGES) & 1);
+      } else if (issued > 0) {
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+      }
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      umma_commit_pair(drain0);
+      mbar_drain(drain0, 0);
+    }
+    __syncthreads();
+  }
+  // neither CTA leaves while the other may still touch its shared memory or TMEM
+  cluster_sync();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * TOK)
+                 : "memory");
+  }
+}
+
+// Adds the K ranges' sums and scales them.
+template <typename S>
+__global__ void __launch_bounds__(256)
+    finish_kernel(S* __restrict__ out, long long ldo, const int32_t* __restrict__ part, int splits,
+                  const float* __restrict__ sa, const float* __restrict__ sb,
+                  const float* __restrict__ bias, long long M, long long N) {
+  for (long long m = blockIdx.y; m < M; m += gridDim.y) {
+    const float s = sa[m];
+    for (long long n = blockIdx.x * 256LL + threadIdx.x; n < N; n += gridDim.x * 256LL) {
+      int acc = 0;
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) acc += part[(k * M + m) * N + n];
+      out[m * ldo + n] = of_f<S>(scaled(acc, s, sb[n], bias ? bias[n] : 0.f));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+static bool byte_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
+                     const cuuint64_t* strides, int box_rows) {
+  auto enc = encode_fn();
+  if (!enc) return false;
+  const cuuint32_t box[3] = {KB, (cuuint32_t)box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box,
+             estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+static long long up16(long long v) { return (v + 15) / 16 * 16; }
+
+bool tc_takes(const Product& p) {
+  return rows::aligned(p.a, 16) && rows::aligned(p.b, 16) && (p.M == 1 || p.lda % 16 == 0) &&
+         (p.N == 1 || p.ldb % 16 == 0) && (p.groups == 1 || p.b_gs % 16 == 0);
+}
+
+constexpr int kClusters = 74;
+
+// K ranges: as many as fill the clusters, each of at least four chunks (half a
+// kilobyte of every row), where there are fewer tiles than clusters.
+static int split_count(const Product& p) {
+  if (p.offsets) return 1;
+  const long long tiles = ((p.M + TOK - 1) / TOK) * ((p.N + CH - 1) / CH);
+  const int nk = cdiv(p.K, KB);
+  long long s = kClusters / tiles;
+  if (s > nk / 4) s = nk / 4;
+  if (s < 2) return 1;
+  // ranges of equal length: as many as that length needs
+  const int per = cdiv(nk, s);
+  return cdiv(nk, per);
+}
+
+size_t tc_workspace_bytes(const Product& p) {
+  if (!tc_takes(p)) return 0;
+  const int s = split_count(p);
+  return s > 1 ? (size_t)s * p.M * p.N * sizeof(int32_t) : 0;
+}
+
+template <typename S>
+static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, cudaStream_t st) {
+  const int smem = STAGES * STAGE_BYTES + 1024 + 128 + 2 * TOK * (int)sizeof(float) +
+                   (int)(3 * a.p.groups + 4) * (int)sizeof(int32_t);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return G2Q_ERR_CUDA;
+  static int attr_done[64] = {0};
+  if (dev >= 64 || !attr_done[dev]) {
+    if (cudaFuncSetAttribute(tc_kernel<S>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             227 * 1024) != cudaSuccess)
+      return G2Q_ERR_CUDA;
+    if (dev < 64) attr_done[dev] = 1;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * (unsigned)(tiles < kClusters ? tiles : kClusters), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tc_kernel<S>, maps[0], maps[1], maps[2], a);
+  g2q::note_launch();
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return G2Q_ERR_CUDA;
+  }
+  if (a.splits > 1) {
+    const unsigned gx = (unsigned)cdiv(a.p.N, 256);
+    const unsigned gy = (unsigned)(a.p.M < 65535 ? a.p.M : 65535);
+    finish_kernel<S><<<dim3(gx, gy), 256, 0, st>>>(static_cast<S*>(a.p.out), a.p.ldo, a.part,
+                                                   a.splits, a.p.sa, a.p.sb, a.p.bias, a.p.M,
+                                                   a.p.N);
+    G2Q_CHECK_LAUNCH();
+  }
+  return G2Q_OK;
+}
+
+int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+  TcArgs a;
+  a.p = p;
+  a.ch_tiles = cdiv(p.N, CH);
+  a.nk = cdiv(p.K, KB);
+  a.splits = split_count(p);
+  a.per_split = cdiv(a.nk, a.splits);
+  a.part = static_cast<int32_t*>(workspace);
+  a.wait_cycles = wait_cycles();
+  const size_t need = tc_workspace_bytes(p);
+  if (need && (!workspace || workspace_bytes < need)) return G2Q_ERR_INVALID_ARG;
+  const long long lda = p.M == 1 ? up16(p.K) : p.lda, ldb = p.N == 1 ? up16(p.K) : p.ldb;
+  const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.groups};
+  const cuuint64_t ws[2] = {(cuuint64_t)ldb, (cuuint64_t)(p.groups > 1 ? p.b_gs : p.N * ldb)};
+  const cuuint64_t td[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
+  const cuuint64_t ts[1] = {(cuuint64_t)lda};
+  CUtensorMap maps[3];
+  if (!byte_map(&maps[0], p.b, 3, wd, ws, 128) || !byte_map(&maps[1], p.a, 2, td, ts, 128) ||
+      !byte_map(&maps[2], p.a, 2, td, ts, 32))
+    return G2Q_ERR_CUDA;
+  const long long tiles = range_slots(p, TOK) * a.ch_tiles * a.splits;
+  if (p.out_dtype == G2Q_DTYPE_BF16) return launch_tc<__nv_bfloat16>(maps, a, tiles, st);
+  if (p.out_dtype == G2Q_DTYPE_F16) return launch_tc<__half>(maps, a, tiles, st);
+  return launch_tc<float>(maps, a, tiles, st);
+}
+
+}  // namespace i8
+}  // namespace g2q

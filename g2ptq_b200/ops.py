@@ -620,9 +620,11 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
     if bias is not None:
         _vector("bias", bias, N)
     out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    ws_bytes = query("g2q_int8_matmul_workspace_bytes", M, N, K)
+    ws = workspace(ws_bytes, dev) if ws_bytes else None
     _call_on(dev, "g2q_int8_matmul", out.data_ptr(), dtype_code(out_dtype), N, a.data_ptr(), lda,
              a_scale.data_ptr(), b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K,
-             _status(None, dev), _stream(a))
+             _ptr(ws), ws_bytes, _status(None, dev), _stream(a))
     return out
 
 

@@ -468,11 +468,15 @@ int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, const void* x,
 /* out[m][n] = a_scale[m] * b_scale[n] * sum_k a[m][k] * b[n][k] + bias[n]:
  * int8 a [M, K] and b [N, K] (row strides lda, ldb), fp32 a_scale [M], b_scale
  * [N] and bias [N] (may be NULL), out [M, N] of type out_dtype (row stride
- * ldo).  The sums are exact 32-bit integers: K above 131071 is unsupported. */
+ * ldo).  The sums are exact 32-bit integers: K above 131071 is unsupported.
+ * Operands whose bases and row strides are multiples of 16 bytes run on the
+ * tensor cores, others on the CUDA cores.  `workspace`:
+ * g2q_int8_matmul_workspace_bytes(M, N, K) bytes (0 for most shapes). */
+size_t g2q_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
                     const float* a_scale, const int8_t* b, int64_t ldb, const float* b_scale,
-                    const float* bias, int64_t M, int64_t N, int64_t K, int* status,
-                    void* stream);
+                    const float* bias, int64_t M, int64_t N, int64_t K, void* workspace,
+                    size_t workspace_bytes, int* status, void* stream);
 
 /* The same for rows sorted into G groups: rows offsets[g] .. offsets[g+1] - 1
  * (device int32 [G + 1], ascending from 0, at most M) use b + g * b_gs and

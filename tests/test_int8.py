@@ -87,14 +87,14 @@ def test_abi_refuses_bad_arguments():
     assert lib.g2q_quantize_tokens(p, 8, p, p, 0, 16, 1, 16, None) == bad
     assert lib.g2q_quantize_tokens(None, 16, None, None, 0, 16, 0, 16, None) == 0
     args = [p, 0, 8, p, 16, p, p, 16, p, None]
-    assert lib.g2q_int8_matmul(*args, 4, 8, 0, None, None) == bad
-    assert lib.g2q_int8_matmul(*args, 4, 9, 16, None, None) == bad  # ldo < N
-    assert lib.g2q_int8_matmul(*args, 4, 8, 17, None, None) == bad  # lda < K
+    assert lib.g2q_int8_matmul(*args, 4, 8, 0, None, 0, None, None) == bad
+    assert lib.g2q_int8_matmul(*args, 4, 9, 16, None, 0, None, None) == bad  # ldo < N
+    assert lib.g2q_int8_matmul(*args, 4, 8, 17, None, 0, None, None) == bad  # lda < K
     args[4] = args[7] = 1 << 20
-    assert lib.g2q_int8_matmul(*args, 4, 8, ops.INT8_MAX_K + 1, None,
+    assert lib.g2q_int8_matmul(*args, 4, 8, ops.INT8_MAX_K + 1, None, 0, None,
                                None) == _lib.G2Q_ERR_UNSUPPORTED
-    assert lib.g2q_int8_matmul(None, 0, 8, None, 16, None, None, 16, None, None, 0, 8, 16, None,
-                               None) == 0
+    assert lib.g2q_int8_matmul(None, 0, 8, None, 16, None, None, 16, None, None, 0, 8, 16, None, 0,
+                               None, None) == 0
     assert lib.g2q_int8_matmul_grouped(p, 0, 8, p, 16, p, p, 16, 128, p, None, 2, 4, 8, 16, None,
                                        None) == bad
     assert lib.g2q_int8_matmul_grouped(p, 0, 8, p, 16, p, p, 16, 128, p, p, 1025, 4, 8, 16, None,
