@@ -292,7 +292,7 @@ static int product(const Product& p, void* workspace, size_t workspace_bytes, cu
 static int check(const Product& p) {
   if (!rows::elem_bytes(p.out_dtype) || p.M < 0 || p.N <= 0 || p.K <= 0 || p.groups <= 0)
     return G2Q_ERR_INVALID_ARG;
-  if (p.K > kMaxK || p.M > 0x7fffffffLL || p.N > 0x7fffffffLL || p.groups > kMaxGroups)
+  if (p.K > kMaxK || p.M > kMaxRows || p.N > kMaxRows || p.groups > kMaxGroups)
     return G2Q_ERR_UNSUPPORTED;
   if (p.M == 0) return G2Q_OK;
   if (!p.out || !p.a || !p.sa || !p.b || !p.sb || p.lda < p.K || p.ldb < p.K || p.ldo < p.N ||
@@ -315,7 +315,9 @@ extern "C" int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, con
 }
 
 extern "C" size_t g2q_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0 || K > i8::kMaxK || M > 0x7fffffffLL || N > 0x7fffffffLL) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || K > i8::kMaxK || M > i8::kMaxRows ||
+      N > i8::kMaxRows)
+    return 0;
   i8::Product p = {};
   p.lda = p.ldb = (K + 15) / 16 * 16;
   p.groups = 1;

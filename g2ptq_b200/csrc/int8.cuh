@@ -8,6 +8,7 @@ namespace i8 {
 
 constexpr long long kMaxK = 131071;     // 128 * 128 * K fits an int32 sum
 constexpr long long kMaxGroups = 1024;  // experts
+constexpr long long kMaxRows = 0x7fff0000LL;  // row and channel indexes stay in 32 bits
 
 // out[m, n] = sa[m] * sb[g, n] * sum_k a[m, k] * b[g, n, k] + bias[n], with
 // g the group of row m: rows offsets[g] .. offsets[g + 1] - 1 (offsets NULL:

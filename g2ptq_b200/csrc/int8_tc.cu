@@ -32,7 +32,7 @@ using namespace g2q::tc;
 using rows::of_f;
 
 constexpr int CH = 256;              // channels per tile (128 per CTA)
-constexpr int TOK = 256;             // most tokens per tile
+constexpr int TOK = 256;             // most tokens per tile, and columns per TMEM buffer
 constexpr int KB = 128;              // bytes of K per operand chunk (one swizzled row)
 constexpr int KC = 2;                // chunks per pipeline stage
 constexpr int OP_BYTES = 128 * KB;   // one operand's chunk in one CTA
@@ -40,10 +40,12 @@ constexpr int STAGE_BYTES = KC * 2 * OP_BYTES;
 constexpr int STAGES = 3;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int STRIP_BYTES = 16 * (32 * 4 + 16);  // 16 tokens x 32 channels, padded
 constexpr int RASTER = 8;            // row pieces walked together
 
 struct TcArgs {
   Product p;
+  int tok;                       // tokens per tile: 64, 128 or 256
   int ch_tiles, nk;              // channel tiles; chunks of K
   int splits, per_split;         // K ranges and chunks in each
   int32_t* part;                 // [splits][M][N] when splits > 1
@@ -52,9 +54,8 @@ struct TcArgs {
 
 // What one cluster works on
 struct Tile {
-  long long row0;
-  int rows, group, ch0, k0, k1;  // k: chunks
-  int split;
+  int row0, rows, group, ch0;
+  int k0, k1, split;  // K range in chunks
 };
 
 // In shared memory: the first piece of each group and the groups' bounds, so
@@ -65,7 +66,7 @@ struct Table {
   int32_t* hi;
 };
 
-__device__ __forceinline__ void build_table(const Product& p, const Table& t) {
+__device__ __forceinline__ void build_table(const Product& p, int tok, const Table& t) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   for (int g0 = 0; g0 <= p.groups; g0 += 32) {
@@ -81,7 +82,7 @@ __device__ __forceinline__ void build_table(const Product& p, const Table& t) {
       t.lo[g] = (int)lo;
       t.hi[g] = (int)hi;
     }
-    const int mine = (int)((hi - lo + TOK - 1) / TOK);
+    const int mine = ((int)(hi - lo) + tok - 1) / tok;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -94,26 +95,29 @@ __device__ __forceinline__ void build_table(const Product& p, const Table& t) {
   if (lane == 0) t.first[p.groups + 1] = before;
 }
 
-__device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, long long w) {
+__device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, int w) {
   Tile r;
-  r.split = (int)(w % a.splits);
-  w /= a.splits;
-  const int pieces = t.first[a.p.groups + 1];
-  const int r0 = (int)(w / ((long long)RASTER * a.ch_tiles)) * RASTER;
+  r.split = 0;
+  if (a.splits > 1) {
+    r.split = w % a.splits;
+    w /= a.splits;
+  }
+  const int groups = (int)a.p.groups, pieces = t.first[groups + 1];
+  const int r0 = w / (RASTER * a.ch_tiles) * RASTER;
   const int gsz = pieces - r0 < RASTER ? pieces - r0 : RASTER;
-  const int rem = (int)(w - (long long)r0 * a.ch_tiles);
+  const int rem = w - r0 * a.ch_tiles;
   const int piece = r0 + rem % gsz;
   r.ch0 = rem / gsz * CH;
-  int lo = 0, hi = (int)a.p.groups;  // the last group with first <= piece
+  int lo = 0, hi = groups;  // the last group with first <= piece
   while (lo < hi) {
     const int mid = (lo + hi + 1) / 2;
     if (t.first[mid] <= piece) lo = mid;
     else hi = mid - 1;
   }
   r.group = lo;
-  r.row0 = t.lo[lo] + (long long)(piece - t.first[lo]) * TOK;
-  const long long left = t.hi[lo] - r.row0;
-  r.rows = (int)(left < TOK ? left : TOK);
+  r.row0 = t.lo[lo] + (piece - t.first[lo]) * a.tok;
+  const int left = t.hi[lo] - r.row0;
+  r.rows = left < a.tok ? left : a.tok;
   r.k0 = r.split * a.per_split;
   r.k1 = r.k0 + a.per_split < a.nk ? r.k0 + a.per_split : a.nk;
   return r;
@@ -152,38 +156,36 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
-template <typename S>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  S v[2] = {of_f<S>(a), of_f<S>(b)};
-  return *reinterpret_cast<uint32_t*>(v);
-}
-
-// 32 columns (tokens) of this lane's channel into out; the warp's 32 lanes are
-// 32 neighbouring channels.  16-bit outputs go two channels at a time: lane
-// pairs exchange so that the even lane holds both channels of the even token,
-// the odd lane both of the odd token.
-template <typename S>
-__device__ __forceinline__ void store_block(S* out, long long ldo, const float* sa, int rows,
-                                            const uint32_t (&r)[32], float sb, float bias,
-                                            long long n, long long N, bool paired, bool zero) {
+// Sixteen tokens (columns) of a warp's 32 channels to memory: dst points at the
+// first token's row and the strip's first channel, `n` channels and `rows`
+// tokens of it exist.  Each lane holds one channel, so the values pass through a
+// padded strip of shared memory to leave as 16-byte pieces of token rows.
+template <typename T>
+__device__ __forceinline__ void store16(T* dst, long long ld, int rows, long long n, bool vec,
+                                        uint8_t* strip, const T (&v)[16]) {
+  constexpr int PITCH = 32 * (int)sizeof(T) + 16;
+  constexpr int PER = 16 / (int)sizeof(T);  // elements per piece
+  constexpr int PIECES = 32 / PER;          // pieces per token
   const int lane = threadIdx.x & 31;
-  if (sizeof(S) == 2 && paired) {
-    const int odd = lane & 1;
-    S* dst = out + odd * ldo + (n - odd);
-    const bool in = n - odd + 1 < N;
+  if (vec) {
 #pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-      float v0 = zero ? 0.f : scaled((int)r[c], sa[c], sb, bias);
-      float v1 = zero ? 0.f : scaled((int)r[c + 1], sa[c + 1], sb, bias);
-      const float other = __shfl_xor_sync(0xffffffffu, odd ? v0 : v1, 1);
-      const uint32_t w = odd ? pack2<S>(other, v1) : pack2<S>(v0, other);
-      if (in && c + odd < rows) *reinterpret_cast<uint32_t*>(dst + c * ldo) = w;
+    for (int c = 0; c < 16; ++c) reinterpret_cast<T*>(strip + c * PITCH)[lane] = v[c];
+    __syncwarp();
+    const int piece = lane % PIECES;
+    T* d = dst + (lane / PIECES) * ld + piece * PER;
+    const bool in = piece * PER < n;
+#pragma unroll
+    for (int i = 0; i < 16 * PIECES / 32; ++i) {
+      const int c = i * (32 / PIECES) + lane / PIECES;
+      if (in && c < rows)
+        *reinterpret_cast<uint4*>(d + (long long)i * (32 / PIECES) * ld) =
+            *reinterpret_cast<const uint4*>(strip + c * PITCH + piece * 16);
     }
+    __syncwarp();
   } else {
 #pragma unroll
-    for (int c = 0; c < 32; ++c)
-      if (n < N && c < rows)
-        out[c * ldo + n] = of_f<S>(zero ? 0.f : scaled((int)r[c], sa[c], sb, bias));
+    for (int c = 0; c < 16; ++c)
+      if (lane < n && c < rows) dst[c * ld + lane] = v[c];
   }
 }
 
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  float* sa_s = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES + 128);  // [2][TOK]
+  uint8_t* strips = smem + STAGES * STAGE_BYTES + 128;  // [EPI_WARPS][STRIP_BYTES]
+  float* sa_s = reinterpret_cast<float*>(strips + EPI_WARPS * STRIP_BYTES);  // [2][TOK]
   Table table;
   table.first = reinterpret_cast<int32_t*>(sa_s + 2 * TOK);
   table.lo = table.first + p.groups + 2;
@@ -234,26 +237,26 @@ __global__ void __launch_bounds__(THREADS, 1)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   } else if (warp == 2) {
-    build_table(p, table);
+    build_table(p, a.tok, table);
   }
   fence_before();
   __syncthreads();
   cluster_sync();  // barriers of both CTAs initialised, TMEM allocated in both
   fence_after();
   const uint32_t tmem = *tmem_holder;
-  const long long total = (long long)table.first[p.groups + 1] * a.ch_tiles * a.splits;
-  const long long step = gridDim.x >> 1;
+  const int total = table.first[p.groups + 1] * a.ch_tiles * a.splits;
+  const int step = gridDim.x >> 1;
 
   int issued = 0;  // stages whose loads this CTA's producer issued
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t full_lead = mapa_shared(full0, 0);
       bool ok = true;
-      for (long long w = blockIdx.x >> 1; ok && w < total; w += step) {
+      for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
         const Tile t = decode(a, table, w);
         if (t.group == p.groups) continue;
         const int half = mma_n(t.rows) / 2;
-        const int y = (int)t.row0 + (int)rank * half;
+        const int y = t.row0 + (int)rank * half;
         const int ych = t.ch0 + 128 * (int)rank;
         for (int k = t.k0; k < t.k1; k += KC) {
           const int s = issued % STAGES;
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (lane == 0 && rank == 0) {
       int it = 0, tc = 0;
       bool ok = true;
-      for (long long w = blockIdx.x >> 1; ok && w < total; w += step) {
+      for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
         const Tile t = decode(a, table, w);
         if (t.group == p.groups) continue;
         const int buf = tc & 1;
@@ -321,20 +324,34 @@ __global__ void __launch_bounds__(THREADS, 1)
     // warps of a quadrant take alternate blocks of 32 tokens
     const int q = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
     const uint32_t acce_lead = mapa_shared(acce0, 0);
+    uint8_t* strip = strips + (warp - 2) * STRIP_BYTES;
     S* out = static_cast<S*>(p.out);
-    const bool paired = (reinterpret_cast<uintptr_t>(out) & 3) == 0 && p.ldo % 2 == 0 &&
-                        p.N % 2 == 0;
-    int tc = 0, turn = 0;
+    const bool vec = a.splits > 1 ? p.N % 4 == 0
+                                  : (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
+                                        p.ldo * sizeof(S) % 16 == 0 && p.N * sizeof(S) % 16 == 0;
+    Tile t, next;
+    float sa_next = 0.f, sb_next = 0.f, bias_next = 0.f;
+    // a tile's scales are loaded one tile ahead; zeros where there is no such
+    // row or channel, and for rows behind the last group
+    auto fetch = [&](int w) {
+      next = decode(a, table, w);
+      const bool zero = next.group == p.groups;
+      const int n = next.ch0 + 128 * (int)rank + q * 32 + lane;
+      sa_next = !zero && et < next.rows ? p.sa[next.row0 + et] : 0.f;
+      sb_next = !zero && n < p.N ? p.sb[(long long)next.group * p.N + n] : 0.f;
+      bias_next = p.bias && n < p.N ? p.bias[n] : 0.f;
+    };
+    int tc = 0, turn = 0, w = blockIdx.x >> 1;
     bool ok = true;
-    for (long long w = blockIdx.x >> 1; w < total; w += step, ++turn) {
-      const Tile t = decode(a, table, w);
-      const bool zero = t.group == p.groups;
-      const long long n = t.ch0 + 128 * (int)rank + q * 32 + lane;
+    if (w < total) fetch(w);
+    for (; w < total; w += step, ++turn) {
+      t = next;
+      const float sb = sb_next, bias = bias_next;
       float* sa = sa_s + (turn & 1) * TOK;
-      sa[et] = et < t.rows ? p.sa[t.row0 + et] : 0.f;
-      const float sb = !zero && n < p.N ? p.sb[(long long)t.group * p.N + n] : 0.f;
-      const float bias = p.bias && n < p.N ? p.bias[n] : 0.f;
+      sa[et] = sa_next;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+      if (w + step < total) fetch(w + step);
+      const bool zero = t.group == p.groups;
       const int buf = tc & 1;
       if (!zero) {
         const uint32_t use_ph = (uint32_t)((tc >> 1) & 1);
@@ -344,18 +361,40 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_after();
       }
       const uint32_t base = tmem + (uint32_t)(buf * TOK) + ((uint32_t)(q * 32) << 16);
+      const long long n0 = t.ch0 + 128 * (long long)rank + q * 32;
+      const long long n = p.N - n0;  // channels of the strip (may be none)
       for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
         uint32_t r[32];
-        if (!zero) tmem_ld32(base + (uint32_t)c0, r);
-        if (!ok) continue;
-        if (a.splits > 1) {
-          int32_t* dst = a.part + ((long long)t.split * p.M + t.row0 + c0) * p.N + n;
+        if (zero) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (n < p.N && c0 + c < t.rows) dst[c * p.N] = (int)r[c];
+          for (int c = 0; c < 32; ++c) r[c] = 0;
         } else {
-          store_block<S>(out + (t.row0 + c0) * p.ldo, p.ldo, sa + c0, t.rows - c0, r, sb, bias, n,
-                         p.N, paired, zero);
+          tmem_ld32(base + (uint32_t)c0, r);
+        }
+        if (!ok) continue;
+#pragma unroll
+        for (int h = 0; h < 32; h += 16) {
+          const long long row = t.row0 + c0 + h;
+          const int rows = t.rows - c0 - h;
+          if (rows <= 0) break;
+          if (a.splits > 1) {
+            int v[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) v[c] = (int)r[h + c];
+            store16<int>(a.part + ((long long)t.split * p.M + row) * p.N + n0, p.N, rows, n, vec,
+                         strip, v);
+          } else {
+            S v[16];
+#pragma unroll
+            for (int c4 = 0; c4 < 16; c4 += 4) {
+              const float4 s4 = *reinterpret_cast<const float4*>(sa + c0 + h + c4);
+              v[c4] = of_f<S>(scaled((int)r[h + c4], s4.x, sb, bias));
+              v[c4 + 1] = of_f<S>(scaled((int)r[h + c4 + 1], s4.y, sb, bias));
+              v[c4 + 2] = of_f<S>(scaled((int)r[h + c4 + 2], s4.z, sb, bias));
+              v[c4 + 3] = of_f<S>(scaled((int)r[h + c4 + 3], s4.w, sb, bias));
+            }
+            store16<S>(out + row * p.ldo + n0, p.ldo, rows, n, vec, strip, v);
+          }
         }
       }
       if (!zero) {
@@ -434,29 +473,56 @@ bool tc_takes(const Product& p) {
 
 constexpr int kClusters = 74;
 
-// K ranges: as many as fill the clusters, each of at least four chunks (half a
-// kilobyte of every row), where there are fewer tiles than clusters.
-static int split_count(const Product& p) {
-  if (p.offsets) return 1;
-  const long long tiles = ((p.M + TOK - 1) / TOK) * ((p.N + CH - 1) / CH);
+// Tokens per tile and K ranges.  Estimated SM cycles of one tile's range: per
+// 128-byte chunk of K the larger of the MMAs' (2 cycles per token column) and of
+// fetching the CTA's operands from L2 (about 48 bytes per cycle), plus the
+// start of a tile and its epilogue; a wave is one range per cluster.  Cutting K
+// adds the finishing kernel and the sums' way through L2.  Few tokens and a
+// short K come out at small tiles, few tiles and a long K at several ranges.
+struct Shape {
+  int tok, splits, per;
+};
+
+static Shape choose(const Product& p) {
   const int nk = cdiv(p.K, KB);
-  long long s = kClusters / tiles;
-  if (s > nk / 4) s = nk / 4;
-  if (s < 2) return 1;
-  // ranges of equal length: as many as that length needs
-  const int per = cdiv(nk, s);
-  return cdiv(nk, per);
+  const long long ch = (p.N + CH - 1) / CH;
+  Shape best = {TOK, 1, nk};
+  if (p.offsets) {
+    // the pieces are only known on the device: tiles that an average group fills
+    const long long avg = p.M / p.groups;
+    best.tok = avg > 128 ? 256 : (avg > 64 ? 128 : 64);
+    return best;
+  }
+  double least = 1e300;
+  for (int tok = 64; tok <= TOK; tok *= 2) {
+    const long long tiles = ((p.M + tok - 1) / tok) * ch;
+    for (int want = 1; want <= 16; ++want) {
+      const int per = (nk + want - 1) / want, s = (nk + per - 1) / per;
+      if (s != want || (want > 1 && per < 4)) continue;
+      const double fetch = (128.0 + tok / 2) * KB / 48.0, mma = 2.0 * tok;
+      const double chunk = fetch > mma ? fetch : mma;
+      const double waves = (double)((tiles * s + kClusters - 1) / kClusters);
+      double cost = waves * (per * chunk + 600.0 + 4.0 * tok);
+      if (s > 1) cost += 4000.0 + (double)p.M * p.N * (s + 1) * 4.0 / (148 * 24.0);
+      if (cost < least) {
+        least = cost;
+        best = {tok, s, per};
+      }
+    }
+  }
+  return best;
 }
 
 size_t tc_workspace_bytes(const Product& p) {
   if (!tc_takes(p)) return 0;
-  const int s = split_count(p);
+  const int s = choose(p).splits;
   return s > 1 ? (size_t)s * p.M * p.N * sizeof(int32_t) : 0;
 }
 
 template <typename S>
 static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, cudaStream_t st) {
-  const int smem = STAGES * STAGE_BYTES + 1024 + 128 + 2 * TOK * (int)sizeof(float) +
+  const int smem = STAGES * STAGE_BYTES + 1024 + 128 + EPI_WARPS * STRIP_BYTES +
+                   2 * TOK * (int)sizeof(float) +
                    (int)(3 * a.p.groups + 4) * (int)sizeof(int32_t);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return G2Q_ERR_CUDA;
@@ -501,12 +567,15 @@ int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaSt
   a.p = p;
   a.ch_tiles = cdiv(p.N, CH);
   a.nk = cdiv(p.K, KB);
-  a.splits = split_count(p);
-  a.per_split = cdiv(a.nk, a.splits);
+  const Shape shape = choose(p);
+  a.tok = shape.tok;
+  a.splits = shape.splits;
+  a.per_split = shape.per;
   a.part = static_cast<int32_t*>(workspace);
   a.wait_cycles = wait_cycles();
   const size_t need = tc_workspace_bytes(p);
-  if (need && (!workspace || workspace_bytes < need)) return G2Q_ERR_INVALID_ARG;
+  if (need && (!workspace || workspace_bytes < need || !rows::aligned(workspace, 16)))
+    return G2Q_ERR_INVALID_ARG;
   const long long lda = p.M == 1 ? up16(p.K) : p.lda, ldb = p.N == 1 ? up16(p.K) : p.ldb;
   const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.groups};
   const cuuint64_t ws[2] = {(cuuint64_t)ldb, (cuuint64_t)(p.groups > 1 ? p.b_gs : p.N * ldb)};
@@ -516,7 +585,8 @@ int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaSt
   if (!byte_map(&maps[0], p.b, 3, wd, ws, 128) || !byte_map(&maps[1], p.a, 2, td, ts, 128) ||
       !byte_map(&maps[2], p.a, 2, td, ts, 32))
     return G2Q_ERR_CUDA;
-  const long long tiles = range_slots(p, TOK) * a.ch_tiles * a.splits;
+  const long long tiles = range_slots(p, a.tok) * a.ch_tiles * a.splits;
+  if (tiles > 0x3fffffffLL) return G2Q_ERR_UNSUPPORTED;
   if (p.out_dtype == G2Q_DTYPE_BF16) return launch_tc<__nv_bfloat16>(maps, a, tiles, st);
   if (p.out_dtype == G2Q_DTYPE_F16) return launch_tc<__half>(maps, a, tiles, st);
   return launch_tc<float>(maps, a, tiles, st);
