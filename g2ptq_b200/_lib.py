@@ -96,6 +96,9 @@ SIGNATURES = {
     "g2q_int8_matmul_workspace_bytes": [I64, I64, I64],
     "g2q_int8_matmul_grouped": [P, I32, I64, P, I64, P, P, I64, I64, P, P, I64, I64, I64, I64, P,
                                 P],
+    "g2q_int8_linear": [P, I32, I64, P, I32, I64, P, I64, I64, P, P, P, I64, I64, I64, I64, P, SZ,
+                        P, P],
+    "g2q_int8_linear_workspace_bytes": [I64, I64, I64, I64],
     "g2q_route": [P, P, P, P, I32, I64, I64, P, SZ, P],
     "g2q_route_workspace_bytes": [I64, I64],
     "g2q_dispatch_rows": [P, I64, P, I64, I32, P, I64, I64, I64, P],
@@ -113,6 +116,7 @@ _RESTYPES = {
     "g2q_gemm_tc_workspace_bytes": SZ,
     "g2q_gram_static_scratch_bytes": SZ,
     "g2q_int8_matmul_workspace_bytes": SZ,
+    "g2q_int8_linear_workspace_bytes": SZ,
     "g2q_route_workspace_bytes": SZ,
 }
 

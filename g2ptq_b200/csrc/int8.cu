@@ -7,8 +7,9 @@
 // The sums are exact in 32-bit integers (|q w| <= 128 * 128, C <= 131071); the
 // only roundings are the conversion of the sum to fp32, the two scalings, the
 // bias and the output type.
-#include "rows.cuh"
 #include "int8.cuh"
+#include "rows.cuh"
+#include "tc_ptx.cuh"
 
 namespace g2q {
 namespace i8 {
@@ -101,6 +102,7 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
                     bool qvec) {
   constexpr int BLOCK = G > 128 ? G : 128;
   constexpr int PER = BLOCK / G;  // rows per block
+  tc::launch_dependents();  // a product that overlaps waits for this kernel to end
   const int tid = threadIdx.x % G;
   const long long t = blockIdx.x * (long long)PER + threadIdx.x / G;
   const bool live = t < T;
@@ -285,8 +287,17 @@ static int simt_product(const Product& p, cudaStream_t st) {
   return G2Q_OK;
 }
 
-static int product(const Product& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
-  return tc_takes(p) ? tc_product(p, workspace, workspace_bytes, st) : simt_product(p, st);
+static int product(const Product& p, void* workspace, size_t workspace_bytes, bool overlap,
+                   cudaStream_t st) {
+  return tc_takes(p) ? tc_product(p, workspace, workspace_bytes, overlap, st) : simt_product(p, st);
+}
+
+static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
+
+// Workspace of a linear: the tokens' codes, their scales, the product's own.
+static size_t linear_workspace(const Product& p) {
+  const size_t M = (size_t)p.M, ld = (size_t)((p.K + 15) / 16 * 16);
+  return up256(M * ld) + up256(M * sizeof(float)) + tc_workspace_bytes(p);
 }
 
 static int check(const Product& p) {
@@ -336,7 +347,7 @@ extern "C" int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8
                    M, N, K, status};
   G2Q_TRY(i8::check(p));
   if (M == 0) return G2Q_OK;
-  return i8::product(p, workspace, workspace_bytes, (cudaStream_t)stream);
+  return i8::product(p, workspace, workspace_bytes, false, (cudaStream_t)stream);
 }
 
 extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t* a,
@@ -349,5 +360,48 @@ extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, co
   if (!offsets) return G2Q_ERR_INVALID_ARG;
   G2Q_TRY(i8::check(p));
   if (M == 0) return G2Q_OK;
-  return i8::product(p, nullptr, 0, (cudaStream_t)stream);
+  return i8::product(p, nullptr, 0, false, (cudaStream_t)stream);
+}
+
+extern "C" size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G) {
+  if (M <= 0 || N <= 0 || K <= 0 || G < 0 || K > i8::kMaxK || M > i8::kMaxRows ||
+      N > i8::kMaxRows || G > i8::kMaxGroups)
+    return 0;
+  i8::Product p = {};
+  p.lda = p.ldb = (K + 15) / 16 * 16;
+  p.b_gs = p.ldb * N;
+  p.groups = G > 0 ? G : 1;
+  p.offsets = G > 0 ? reinterpret_cast<const int32_t*>(16) : nullptr;  // only whether there are any
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  return i8::linear_workspace(p);
+}
+
+extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void* x, int x_dtype,
+                               int64_t ldx, const int8_t* b, int64_t ldb, int64_t b_gs,
+                               const float* b_scale, const float* bias, const int32_t* offsets,
+                               int64_t G, int64_t M, int64_t N, int64_t K, void* workspace,
+                               size_t workspace_bytes, int* status, void* stream) {
+  const int64_t ld = (K + 15) / 16 * 16;
+  if (!rows::elem_bytes(x_dtype) || ldx < K || G < 0 || (G > 0) != (offsets != nullptr) ||
+      (G > 0 && bias))
+    return G2Q_ERR_INVALID_ARG;
+  // the operands that the workspace will hold stand in for the check
+  i8::Product p = {out, out_dtype, ldo, static_cast<int8_t*>(workspace), ld,
+                   static_cast<float*>(workspace), b, ldb, b_gs, b_scale, bias, offsets,
+                   G > 0 ? G : 1, M, N, K, status};
+  G2Q_TRY(i8::check(p));
+  if (M == 0) return G2Q_OK;
+  if (!x || !rows::aligned(workspace, 16) || workspace_bytes < i8::linear_workspace(p))
+    return G2Q_ERR_INVALID_ARG;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const size_t code_bytes = i8::up256((size_t)M * (size_t)ld);
+  const size_t scale_bytes = i8::up256((size_t)M * sizeof(float));
+  float* scale = reinterpret_cast<float*>(ws + code_bytes);
+  p.sa = scale;
+  G2Q_TRY(i8::quantize_tokens(reinterpret_cast<int8_t*>(ws), ld, scale, x, x_dtype, ldx, M, K,
+                              (cudaStream_t)stream));
+  return i8::product(p, ws + code_bytes + scale_bytes, workspace_bytes - code_bytes - scale_bytes,
+                     true, (cudaStream_t)stream);
 }

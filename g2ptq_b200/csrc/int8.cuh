@@ -96,10 +96,13 @@ __device__ __forceinline__ float scaled(int acc, float sa, float sb, float bias)
 }
 
 // The tensor-core product (int8_tc.cu): whether it takes these operands (bases
-// and row strides multiples of 16 bytes), the workspace it needs, the launch.
+// and row strides multiples of 16 bytes), the workspace it needs, the launch
+// (`overlap`: it may start while the stream's last kernel, which wrote a and
+// sa and nothing else that it reads, is still running).
 bool tc_takes(const Product& p);
 size_t tc_workspace_bytes(const Product& p);
-int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaStream_t st);
+int tc_product(const Product& p, void* workspace, size_t workspace_bytes, bool overlap,
+               cudaStream_t st);
 
 }  // namespace i8
 }  // namespace g2q

@@ -247,38 +247,56 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int total = table.first[p.groups + 1] * a.ch_tiles * a.splits;
   const int step = gridDim.x >> 1;
 
+  launch_dependents();  // the finishing kernel, which waits for this one to end
   int issued = 0;  // stages whose loads this CTA's producer issued
   if (warp == 0) {
     if (lane == 0) {
       const uint32_t full_lead = mapa_shared(full0, 0);
-      bool ok = true;
+      // loads of chunks k .. of tile t into stage s: the weight's, the tokens'
+      auto load_w = [&](const Tile& t, int k, int s) {
+        const int nc = t.k1 - k < KC ? t.k1 - k : KC, half = mma_n(t.rows) / 2;
+        // the leader's full[s] expects the bytes of both CTAs
+        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * nc * (OP_BYTES + half * KB));
+        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+        for (int c = 0; c < nc; ++c)
+          tma_load_3d_pair(st + c * OP_BYTES, &mw, (k + c) * KB, t.ch0 + 128 * (int)rank, t.group,
+                           full_lead + 8 * s);
+      };
+      auto load_t = [&](const Tile& t, int k, int s) {
+        const int nc = t.k1 - k < KC ? t.k1 - k : KC, half = mma_n(t.rows) / 2;
+        const int y = t.row0 + (int)rank * half;
+        const uint32_t fb = full_lead + 8 * s;
+        for (int c = 0; c < nc; ++c) {
+          const uint32_t sb = smem_u32(smem + s * STAGE_BYTES) + (KC + c) * OP_BYTES;
+          const int x = (k + c) * KB;
+          if (half == 128) {
+            tma_load_2d_pair(sb, &mt128, x, y, fb);
+          } else {
+            for (int i = 0; i < half; i += 32) tma_load_2d_pair(sb + i * KB, &mt32, x, y + i, fb);
+          }
+        }
+      };
+      bool ok = true, first = true;
       for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
         const Tile t = decode(a, table, w);
         if (t.group == p.groups) continue;
-        const int half = mma_n(t.rows) / 2;
-        const int y = t.row0 + (int)rank * half;
-        const int ych = t.ch0 + 128 * (int)rank;
-        for (int k = t.k0; k < t.k1; k += KC) {
+        int k = t.k0;
+        if (first) {
+          // the weight does not depend on the kernel before this one (the tokens'
+          // quantization): its first stages are on their way while that ends
+          for (; issued < STAGES && k < t.k1; k += KC) load_w(t, k, issued++);
+          wait_predecessor();
+          for (int s = 0, kk = t.k0; s < issued; ++s, kk += KC) load_t(t, kk, s);
+          first = false;
+        }
+        for (; k < t.k1; k += KC) {
           const int s = issued % STAGES;
           const uint32_t ph = (issued / STAGES) & 1;
           ok = mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, a.wait_cycles);
           if (!ok) break;
           ++issued;
-          const int nc = t.k1 - k < KC ? t.k1 - k : KC;
-          // the leader's full[s] expects the bytes of both CTAs
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * nc * (OP_BYTES + half * KB));
-          const uint32_t fb = full_lead + 8 * s;
-          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-          for (int c = 0; c < nc; ++c) {
-            const int x = (k + c) * KB;
-            tma_load_3d_pair(st + c * OP_BYTES, &mw, x, ych, t.group, fb);
-            const uint32_t sb = st + (KC + c) * OP_BYTES;
-            if (half == 128) {
-              tma_load_2d_pair(sb, &mt128, x, y, fb);
-            } else {
-              for (int i = 0; i < half; i += 32) tma_load_2d_pair(sb + i * KB, &mt32, x, y + i, fb);
-            }
-          }
+          load_w(t, k, s);
+          load_t(t, k, s);
         }
       }
     }
@@ -343,6 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     };
     int tc = 0, turn = 0, w = blockIdx.x >> 1;
     bool ok = true;
+    wait_predecessor();  // the tokens' scales
     if (w < total) fetch(w);
     for (; w < total; w += step, ++turn) {
       t = next;
@@ -438,6 +457,7 @@ __global__ void __launch_bounds__(256)
     finish_kernel(S* __restrict__ out, long long ldo, const int32_t* __restrict__ part, int splits,
                   const float* __restrict__ sa, const float* __restrict__ sb,
                   const float* __restrict__ bias, long long M, long long N) {
+  wait_predecessor();
   for (long long m = blockIdx.y; m < M; m += gridDim.y) {
     const float s = sa[m];
     for (long long n = blockIdx.x * 256LL + threadIdx.x; n < N; n += gridDim.x * 256LL) {
@@ -520,7 +540,8 @@ size_t tc_workspace_bytes(const Product& p) {
 }
 
 template <typename S>
-static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, cudaStream_t st) {
+static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, bool overlap,
+                     cudaStream_t st) {
   const int smem = STAGES * STAGE_BYTES + 1024 + 128 + EPI_WARPS * STRIP_BYTES +
                    2 * TOK * (int)sizeof(float) +
                    (int)(3 * a.p.groups + 4) * (int)sizeof(int32_t);
@@ -538,31 +559,38 @@ static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, 
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tc_kernel<S>, maps[0], maps[1], maps[2], a);
+  cfg.numAttrs = overlap ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, tc_kernel<S>, maps[0], maps[1], maps[2], a);
   g2q::note_launch();
+  if (e == cudaSuccess && a.splits > 1) {
+    cudaLaunchConfig_t fin = {};
+    fin.gridDim = dim3((unsigned)cdiv(a.p.N, 256), (unsigned)(a.p.M < 65535 ? a.p.M : 65535), 1);
+    fin.blockDim = dim3(256, 1, 1);
+    fin.stream = st;
+    fin.attrs = attr + 1;
+    fin.numAttrs = 1;
+    e = cudaLaunchKernelEx(&fin, finish_kernel<S>, static_cast<S*>(a.p.out), a.p.ldo,
+                           static_cast<const int32_t*>(a.part), a.splits, a.p.sa, a.p.sb, a.p.bias,
+                           a.p.M, a.p.N);
+    g2q::note_launch();
+  }
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return G2Q_ERR_CUDA;
   }
-  if (a.splits > 1) {
-    const unsigned gx = (unsigned)cdiv(a.p.N, 256);
-    const unsigned gy = (unsigned)(a.p.M < 65535 ? a.p.M : 65535);
-    finish_kernel<S><<<dim3(gx, gy), 256, 0, st>>>(static_cast<S*>(a.p.out), a.p.ldo, a.part,
-                                                   a.splits, a.p.sa, a.p.sb, a.p.bias, a.p.M,
-                                                   a.p.N);
-    G2Q_CHECK_LAUNCH();
-  }
   return G2Q_OK;
 }
 
-int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaStream_t st) {
+int tc_product(const Product& p, void* workspace, size_t workspace_bytes, bool overlap,
+               cudaStream_t st) {
   TcArgs a;
   a.p = p;
   a.ch_tiles = cdiv(p.N, CH);
@@ -587,9 +615,9 @@ int tc_product(const Product& p, void* workspace, size_t workspace_bytes, cudaSt
     return G2Q_ERR_CUDA;
   const long long tiles = range_slots(p, a.tok) * a.ch_tiles * a.splits;
   if (tiles > 0x3fffffffLL) return G2Q_ERR_UNSUPPORTED;
-  if (p.out_dtype == G2Q_DTYPE_BF16) return launch_tc<__nv_bfloat16>(maps, a, tiles, st);
-  if (p.out_dtype == G2Q_DTYPE_F16) return launch_tc<__half>(maps, a, tiles, st);
-  return launch_tc<float>(maps, a, tiles, st);
+  if (p.out_dtype == G2Q_DTYPE_BF16) return launch_tc<__nv_bfloat16>(maps, a, tiles, overlap, st);
+  if (p.out_dtype == G2Q_DTYPE_F16) return launch_tc<__half>(maps, a, tiles, overlap, st);
+  return launch_tc<float>(maps, a, tiles, overlap, st);
 }
 
 }  // namespace i8

@@ -554,6 +554,12 @@ def _call_on(device, name, *args):
         return call(name, *args)
 
 
+def _raw_stream(device):
+    """The current stream of ``device`` as ``_stream`` gives it, without the
+    Stream object (a tenth of a microsecond instead of two)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _matrix(name, t):
     """Row stride of the 2-D ``t`` with unit column stride and rows that do not overlap."""
     if t.dim() != 2:
@@ -597,7 +603,7 @@ def quantize_tokens(x):
     codes = torch.empty(T, ldq, dtype=torch.int8, device=dev)[:, :C]
     scale = torch.empty(T, dtype=torch.float32, device=dev)
     _call_on(dev, "g2q_quantize_tokens", codes.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(),
-             dtype_code(x.dtype), ldx, T, C, _stream(x))
+             dtype_code(x.dtype), ldx, T, C, _raw_stream(dev))
     return codes, scale
 
 
@@ -624,7 +630,7 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
     ws = workspace(ws_bytes, dev) if ws_bytes else None
     _call_on(dev, "g2q_int8_matmul", out.data_ptr(), dtype_code(out_dtype), N, a.data_ptr(), lda,
              a_scale.data_ptr(), b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K,
-             _ptr(ws), ws_bytes, _status(None, dev), _stream(a))
+             _ptr(ws), ws_bytes, _status(None, dev), _raw_stream(dev))
     return out
 
 
@@ -662,7 +668,54 @@ def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat1
     out = torch.empty(R, N, dtype=out_dtype, device=dev)
     _call_on(dev, "g2q_int8_matmul_grouped", out.data_ptr(), dtype_code(out_dtype), N,
              a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb, b_gs, b_scale.data_ptr(),
-             offsets.data_ptr(), b.shape[0], R, N, K, _status(None, dev), _stream(a))
+             offsets.data_ptr(), b.shape[0], R, N, K, _status(None, dev), _raw_stream(dev))
+    return out
+
+
+def int8_linear(x, codes, scale, bias=None):
+    """``quantize_tokens`` of ``x [M, K]`` and ``int8_matmul`` with ``codes [N, K]``
+    in one call; the result has ``x``'s type."""
+    dev = _cuda(x, codes, scale, bias)
+    ldx, ldb = _matrix("x", x), _matrix("codes", codes)
+    if codes.dtype != torch.int8:
+        raise TypeError("int8_linear takes int8 codes")
+    M, K = x.shape
+    N, Kb = codes.shape
+    if Kb != K:
+        raise ValueError(f"x has {K} columns and codes {Kb}")
+    if not 0 < K <= INT8_MAX_K or N == 0:
+        raise ValueError(f"int8_linear needs 1 to {INT8_MAX_K} columns and at least one channel")
+    _vector("scale", scale, N)
+    if bias is not None:
+        _vector("bias", bias, N)
+    dt = dtype_code(x.dtype)
+    out = torch.empty(M, N, dtype=x.dtype, device=dev)
+    ws_bytes = query("g2q_int8_linear_workspace_bytes", M, N, K, 0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call_on(dev, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx,
+             codes.data_ptr(), ldb, 0, scale.data_ptr(), _ptr(bias), None, 0, M, N, K,
+             ws.data_ptr(), ws_bytes, _status(None, dev), _raw_stream(dev))
+    return out
+
+
+def int8_linear_grouped(x, codes, scale, offsets):
+    """``quantize_tokens`` of ``x [R, K]`` and ``int8_matmul_grouped`` with ``codes
+    [E, N, K]`` in one call; the result has ``x``'s type."""
+    dev = _cuda(x, codes, scale, offsets)
+    ldx = _matrix("x", x)
+    if codes.dtype != torch.int8:
+        raise TypeError("int8_linear_grouped takes int8 codes")
+    R, K = x.shape
+    N, ldb, b_gs = _expert_weight(codes, scale, K)
+    E = codes.shape[0]
+    _vector("offsets", offsets, E + 1, torch.int32)
+    dt = dtype_code(x.dtype)
+    out = torch.empty(R, N, dtype=x.dtype, device=dev)
+    ws_bytes = query("g2q_int8_linear_workspace_bytes", R, N, K, E)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    _call_on(dev, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx,
+             codes.data_ptr(), ldb, b_gs, scale.data_ptr(), None, offsets.data_ptr(), E, R, N, K,
+             ws.data_ptr(), ws_bytes, _status(None, dev), _raw_stream(dev))
     return out
 
 
@@ -693,7 +746,7 @@ def route(experts, num_experts):
     ws = workspace(ws_bytes, dev) if ws_bytes else None
     _call_on(dev, "g2q_route", order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
              experts.data_ptr(), int(experts.dtype == torch.int64), n, int(num_experts), _ptr(ws),
-             ws_bytes, _stream(experts))
+             ws_bytes, _raw_stream(dev))
     return order, position, offsets
 
 
@@ -717,7 +770,7 @@ def dispatch_rows(x, position):
         raise TypeError(f"unsupported dtype {x.dtype}")
     out = torch.empty(T * k, x.shape[1], dtype=x.dtype, device=dev)
     _call_on(dev, "g2q_dispatch_rows", out.data_ptr(), x.shape[1], x.data_ptr(), ldx,
-             x.element_size(), position.data_ptr(), T, k, x.shape[1], _stream(x))
+             x.element_size(), position.data_ptr(), T, k, x.shape[1], _raw_stream(dev))
     return out
 
 
@@ -745,7 +798,7 @@ def combine_rows(y, position, weights=None):
     out = torch.empty(T, C, dtype=y.dtype, device=dev)
     _call_on(dev, "g2q_combine_rows", out.data_ptr(), C, y.data_ptr(), ldy, dtype_code(y.dtype),
              position.data_ptr(), _ptr(weights), 0 if weights is None else dtype_code(weights.dtype),
-             T, k, C, _stream(y))
+             T, k, C, _raw_stream(dev))
     return out
 
 
@@ -773,5 +826,5 @@ def combine_rows_backward(grad, y, position, weights, need_y=True, need_weights=
     gw = torch.empty(T, k, dtype=weights.dtype, device=dev) if need_weights else None
     _call_on(dev, "g2q_combine_rows_backward", _ptr(gy), C, _ptr(gw), grad.data_ptr(), ldg,
              _ptr(y), ldy, dtype_code(grad.dtype), position.data_ptr(), weights.data_ptr(),
-             dtype_code(weights.dtype), T, k, C, _stream(grad))
+             dtype_code(weights.dtype), T, k, C, _raw_stream(dev))
     return gy, gw

@@ -28,8 +28,7 @@ def int8_linear(x, codes, scale, bias=None):
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     if x2.shape[1] > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()
-    q, s = ops.quantize_tokens(x2)
-    y = ops.int8_matmul(q, s, codes, scale, bias, out_dtype=x.dtype)
+    y = ops.int8_linear(x2, codes, scale, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
 
 
@@ -40,8 +39,7 @@ def int8_experts(x, codes, scale, offsets):
     expert's give zeros."""
     if x.dim() == 2 and x.shape[1] > 1 and x.stride(1) != 1:
         x = x.contiguous()
-    q, s = ops.quantize_tokens(x)
-    return ops.int8_matmul_grouped(q, s, codes, scale, offsets, out_dtype=x.dtype)
+    return ops.int8_linear_grouped(x, codes, scale, offsets)
 
 
 def weight_codes(weight, quantizer):

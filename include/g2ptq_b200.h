@@ -487,6 +487,17 @@ int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t*
                             const float* b_scale, const int32_t* offsets, int64_t G, int64_t M,
                             int64_t N, int64_t K, int* status, void* stream);
 
+/* g2q_quantize_tokens of x [M, K] (type x_dtype) followed by g2q_int8_matmul
+ * (G = 0, offsets NULL) or g2q_int8_matmul_grouped (G > 0, bias NULL) in one
+ * call, the product starting while the quantization ends.  `workspace`: g2q_int8_linear_workspace_bytes(M, N, K, G) bytes, 16-byte
+ * aligned. */
+size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G);
+int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void* x, int x_dtype, int64_t ldx,
+                    const int8_t* b, int64_t ldb, int64_t b_gs, const float* b_scale,
+                    const float* bias, const int32_t* offsets, int64_t G, int64_t M, int64_t N,
+                    int64_t K, void* workspace, size_t workspace_bytes, int* status,
+                    void* stream);
+
 /* ---- expert routing ----
  * Replaces the per-expert index, gather and index_add of the routed expert
  * forward (utils/models/mixins.py:233-259). */

@@ -383,6 +383,51 @@ def test_int8_linear(dtype, shape, N):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("counts,tail", COUNTS)
+def test_int8_experts(dtype, counts, tail):
+    """One call for quantization and grouped product: the two calls' result."""
+    g = gen(tail)
+    a, _, b, sb, off = grouped_case(counts, tail, 40, 272, 77)
+    x = torch.randn(a.shape, generator=g, device=DEV).to(dtype)
+    got = int8_utils.int8_experts(x, b, sb, off)
+    q, s = ops.quantize_tokens(x)
+    assert torch.equal(got, ops.int8_matmul_grouped(q, s, b, sb, off, out_dtype=dtype))
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_int8_linear_is_its_two_steps(M, N, K):
+    g = gen(M + N + K)
+    x = torch.randn(M, K, generator=g, device=DEV)
+    b, sb = aligned_codes((N, K), g), torch.rand(N, generator=g, device=DEV)
+    q, s = ops.quantize_tokens(x)
+    want = ops.int8_matmul(q, s, b, sb, out_dtype=x.dtype)
+    for _ in range(20):  # back to back: the product overlaps the quantization's end
+        got = int8_utils.int8_linear(x, b, sb)
+    assert torch.equal(got, want)
+    assert torch.equal(ops.int8_linear(x, b.contiguous(), sb), want)  # rows of any alignment
+
+
+@gpu
+def test_int8_linear_refusals():
+    w, s = torch.zeros(3, 4, dtype=torch.int8, device=DEV), torch.ones(3, device=DEV)
+    x = torch.zeros(2, 4, device=DEV)
+    off = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for bad in (lambda: ops.int8_linear(x[:, :3], w, s), lambda: ops.int8_linear(x, w, s[:2]),
+                lambda: ops.int8_linear(x[0], w, s), lambda: ops.int8_linear(x, w, s.half()),
+                lambda: ops.int8_linear(x, w, s, x[0]),
+                lambda: ops.int8_linear_grouped(x, w, s, off),
+                lambda: ops.int8_linear_grouped(x, w[None], s[None], off[:1])):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: ops.int8_linear(x, w.float(), s), lambda: ops.int8_linear(x.double(), w, s),
+                lambda: ops.int8_linear_grouped(x.double(), w[None], s[None], off)):
+        with pytest.raises(TypeError):
+            bad()
+
+
+@gpu
 def test_int8_linear_transposed_input():
     g = gen(4)
     x = torch.randn(64, 30, generator=g, device=DEV).t()
