@@ -26,63 +26,117 @@ constexpr unsigned kInfBits = 0x7f800000u;
 // Sixteen consecutive elements of a row, raw; missing ones (beyond `have`) are zero.
 template <typename S>
 struct Unit {
-  static constexpr int Q = 16 * (int)sizeof(S) / 16;  // 16-byte pieces
-  uint4 raw[Q];
+  static constexpr int W = 16 * (int)sizeof(S) / 4;  // 32-bit words
+  uint32_t raw[W];
 
   __device__ __forceinline__ void load(const S* p, int have, bool vec) {
     if (vec && have >= 16) {
 #pragma unroll
-      for (int i = 0; i < Q; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      for (int i = 0; i < W / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        raw[4 * i] = v.x;
+        raw[4 * i + 1] = v.y;
+        raw[4 * i + 2] = v.z;
+        raw[4 * i + 3] = v.w;
+      }
     } else {
-      S* e = reinterpret_cast<S*>(raw);
+      S e[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) e[i] = i < have ? p[i] : of_f<S>(0.f);
+      memcpy(raw, e, sizeof(raw));
     }
   }
   __device__ __forceinline__ float at(int i) const {
-    return to_f<S>(reinterpret_cast<const S*>(raw)[i]);
+    if constexpr (sizeof(S) == 4) {
+      return __uint_as_float(raw[i]);
+    } else {
+      const uint16_t h = (uint16_t)(raw[i / 2] >> (16 * (i % 2)));
+      S v;
+      memcpy(&v, &h, 2);
+      return to_f<S>(v);
+    }
   }
-  // the largest magnitude as fp32 bits (ordered as unsigned; infinities and
-  // NaN come out at or above kInfBits)
+  // the largest magnitude: the bits of a non-negative number order like an
+  // unsigned integer, infinities and NaN at the top.  16-bit types: the two
+  // halves of a word side by side, merged by top_of.
   __device__ __forceinline__ unsigned top_bits() const {
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(at(i)) & 0x7fffffffu);
+    for (int i = 0; i < W; ++i)
+      m = sizeof(S) == 4 ? max(m, raw[i] & 0x7fffffffu) : __vmaxu2(m, raw[i] & 0x7fff7fffu);
     return m;
   }
 };
 
-// round(v / scale), ties to even, of the real quotient: the product with the
-// rounded reciprocal is within 1e-4 of it (|quotient| <= 127), so its rounding
-// is right unless it lands that near a half-integer h; there the sign of the
-// exactly rounded residual v - h * scale decides.
-__device__ __forceinline__ int code_of(float v, float scale, float inv) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the integer
-  const float t = fmaf(v, inv, kMagic);
-  const float n = t - kMagic;
-  const float d = fmaf(v, inv, -n);
-  if (fabsf(d) > 0.4999f) {
-    const float h = n + copysignf(0.5f, d);
-    const float res = fmaf(-h, scale, v);
-    const float lo = h - 0.5f, hi = h + 0.5f;
-    const float even = (static_cast<int>(lo) & 1) ? hi : lo;
-    return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
+// fp32 bits of the magnitude that top_bits collected
+template <typename S>
+__device__ __forceinline__ unsigned top_of(unsigned m) {
+  if constexpr (sizeof(S) == 4) {
+    return m;
+  } else {
+    const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
+    S v;
+    memcpy(&v, &h, 2);
+    return __float_as_uint(to_f<S>(v));
   }
-  return static_cast<int>(n);
+}
+
+// round(v / scale), ties to even, of the real quotient, for a quotient whose
+// product with the rounded reciprocal lies within 1e-4 of the half-integer h
+// between n and its neighbour: the sign of the exactly rounded residual
+// v - h * scale decides.
+__device__ __forceinline__ int code_near_tie(float v, float scale, float n, float d) {
+  const float h = n + copysignf(0.5f, d);
+  const float res = fmaf(-h, scale, v);
+  const float lo = h - 0.5f, hi = h + 0.5f;
+  const float even = (static_cast<int>(lo) & 1) ? hi : lo;
+  return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
+}
+
+// Codes of a unit, four to a word.  The product with the rounded reciprocal is
+// within 1e-4 of the quotient (of at most 127), so its rounding is the
+// quotient's unless it lands that near a half-integer: then (one unit in some
+// hundreds) the unit's near ties are settled one by one.
+template <typename S>
+__device__ __forceinline__ void unit_codes(const Unit<S>& u, float scale, float inv,
+                                           uint32_t (&w)[4]) {
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the integer's
+  float far = 0.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = u.at(4 * g + i), t = fmaf(v, inv, kMagic), n = t - kMagic;
+      far = fmaxf(far, fabsf(fmaf(v, inv, -n)));
+      b[i] = __float_as_uint(t);
+    }
+    w[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+  }
+  if (far > 0.4999f) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i) {
+      float v = u.at(0);
+#pragma unroll
+      for (int k = 1; k < 16; ++k)
+        if (k == i) v = u.at(k);
+      const float t = fmaf(v, inv, kMagic), n = t - kMagic, d = fmaf(v, inv, -n);
+      if (fabsf(d) > 0.4999f) {
+        const uint32_t code = static_cast<uint32_t>(code_near_tie(v, scale, n, d)) & 255u;
+        const int sh = 8 * (i % 4);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (g == i / 4) w[g] = (w[g] & ~(255u << sh)) | code << sh;
+      }
+    }
+  }
 }
 
 template <typename S>
 __device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int have, bool vec,
                                             float scale, float inv, bool finite) {
-  uint32_t w[4];
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    uint32_t b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      b[i] = finite ? static_cast<uint32_t>(code_of(u.at(4 * g + i), scale, inv)) & 255u : 0u;
-    w[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-  }
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (finite) unit_codes<S>(u, scale, inv, w);
   if (vec && have >= 16) {
     *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -90,6 +144,15 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int h
     for (int i = 0; i < 16; ++i)
       if (i < have) dst[i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
   }
+}
+
+// Scale of a row from its largest magnitude's bits, and the reciprocal; false
+// where a value is not finite, which makes the whole row NaN (codes zero).
+__device__ __forceinline__ bool row_scale(unsigned top, float* scale, float* inv) {
+  *scale = __fdiv_rn(__uint_as_float(top), 127.f);
+  if (*scale < 1.17549435e-38f) *scale = 1.f;  // zeros (and values below the normal range)
+  *inv = __frcp_rn(*scale);
+  return top < kInfBits;
 }
 
 // G threads per row, UNITS units of 16 elements per thread kept in registers
@@ -122,12 +185,12 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
     }
 #pragma unroll
     for (int k = 0; k < UNITS; ++k)
-      if (tid + (long long)k * G < units) top = max(top, u[k].top_bits());
+      if (tid + (long long)k * G < units) top = max(top, top_of<S>(u[k].top_bits()));
     for (long long i = tid + (long long)UNITS * G; i < units; i += G) {
       const long long left = C - 16 * i;
       Unit<S> v;
       v.load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
-      top = max(top, v.top_bits());
+      top = max(top, top_of<S>(v.top_bits()));
     }
   }
   top = __reduce_max_sync(0xffffffffu, top);
@@ -140,11 +203,8 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
     for (int w = 0; w < G / 32; ++w) top = max(top, warp_top[w0 + w]);
   }
   if (!live) return;
-  // a value that is not finite makes its whole row NaN: scale NaN, codes zero
-  const bool finite = top < kInfBits;
-  float scale = __fdiv_rn(__uint_as_float(top), 127.f);
-  if (scale < 1.17549435e-38f) scale = 1.f;  // rows of zeros (and of values below normal range)
-  const float inv = __frcp_rn(scale);
+  float scale, inv;
+  const bool finite = row_scale(top, &scale, &inv);
   if (tid == 0) scale_out[t] = finite ? scale : __uint_as_float(0x7fc00000u);
   int8_t* qrow = codes + t * ldq;
 #pragma unroll

@@ -255,157 +255,192 @@ __device__ __forceinline__ float weight_at(const void* w, int dtype, long long i
   return to_f(static_cast<const __half*>(w)[i]);
 }
 
-constexpr int SLOTS = 8;  // slots whose rows are in flight together
+constexpr int SLOTS = 8;  // most slots whose rows are in flight together
 
-// One lane per piece of a token's row; the slots' pieces are loaded together
-// and added in slot order in fp32.
-template <typename S, int W>
+// Slots j0 .. j0 + KT - 1 of token t, the same in every lane: their rows (-1
+// for none) and weights.
+template <int KT>
+struct Slots {
+  int row[KT];
+  float w[KT];
+
+  __device__ __forceinline__ void load(const int32_t* __restrict__ position,
+                                       const void* __restrict__ weights, int w_dtype, long long t,
+                                       int k, int j0, long long n) {
+    const int lane = threadIdx.x & 31;
+    int r = -1;
+    float v = 0.f;
+    if (lane < KT && j0 + lane < k) {
+      r = position[t * k + j0 + lane];
+      if (r >= n) r = -1;
+      if (r >= 0) v = weight_at(weights, w_dtype, t * k + j0 + lane);
+    }
+#pragma unroll
+    for (int j = 0; j < KT; ++j) {
+      row[j] = __shfl_sync(0xffffffffu, r, j);
+      w[j] = __shfl_sync(0xffffffffu, v, j);
+    }
+  }
+};
+
+// One warp per token (few tokens: per segment of its row, blockIdx.y), U pieces
+// per lane in flight for each of KT slots, added in slot order in fp32.  MANY:
+// more than KT slots, in rounds.
+template <typename S, int W, int KT, int U, bool MANY>
 __global__ void __launch_bounds__(256)
     combine_kernel(S* __restrict__ out, long long ldo, const S* __restrict__ y, long long ldy,
                    const int32_t* __restrict__ position, const void* __restrict__ w, int w_dtype,
-                   long long T, int k, long long n, long long pieces, long long segs) {
+                   long long T, int k, long long n, int pieces) {
   using L = Elems<S, W>;
   using V = typename L::V;
   const int lane = threadIdx.x & 31;
-  const long long warps = (long long)gridDim.x * 8;
-  for (long long item = blockIdx.x * 8LL + (threadIdx.x >> 5); item < T * segs; item += warps) {
-    const long long t = item / segs;
-    const long long piece = (item - t * segs) * 32 + lane;
-    const bool live = piece < pieces;
-    float acc[L::N];
+  for (long long t = blockIdx.x * 8LL + (threadIdx.x >> 5); t < T; t += gridDim.x * 8LL) {
+    Slots<KT> s;
+    if (!MANY) s.load(position, w, w_dtype, t, k, 0, n);
+    for (int p0 = blockIdx.y * (32 * U); p0 < pieces; p0 += gridDim.y * (32 * U)) {
+      float acc[U][L::N];
 #pragma unroll
-    for (int u = 0; u < L::N; ++u) acc[u] = 0.f;
-    for (int j0 = 0; j0 < k; j0 += SLOTS) {
-      // lane j holds slot j0 + j's row and weight
-      int row = -1;
-      float wt = 0.f;
-      if (lane < SLOTS && j0 + lane < k) {
-        row = position[t * k + j0 + lane];
-        if (row >= n) row = -1;
-        if (row >= 0) wt = weight_at(w, w_dtype, t * k + j0 + lane);
-      }
-      V v[SLOTS];
-      int r[SLOTS];
+      for (int i = 0; i < U; ++i)
 #pragma unroll
-      for (int j = 0; j < SLOTS; ++j) {
-        r[j] = __shfl_sync(0xffffffffu, row, j);
-        if (live && r[j] >= 0) v[j] = reinterpret_cast<const V*>(y + r[j] * ldy)[piece];
-      }
+        for (int u = 0; u < L::N; ++u) acc[i][u] = 0.f;
+      for (int j0 = 0; j0 < (MANY ? k : 1); j0 += KT) {
+        if (MANY) s.load(position, w, w_dtype, t, k, j0, n);
+        V v[KT][U];
 #pragma unroll
-      for (int j = 0; j < SLOTS; ++j) {
-        const float wj = __shfl_sync(0xffffffffu, wt, j);
-        if (live && r[j] >= 0) {
-          float f[L::N];
-          L::load(f, v[j]);
+        for (int j = 0; j < KT; ++j)
 #pragma unroll
-          for (int u = 0; u < L::N; ++u) acc[u] = fmaf(wj, f[u], acc[u]);
+          for (int i = 0; i < U; ++i) {
+            const int p = p0 + 32 * i + lane;
+            if (p < pieces && s.row[j] >= 0)
+              v[j][i] = reinterpret_cast<const V*>(y + s.row[j] * ldy)[p];
+          }
+#pragma unroll
+        for (int j = 0; j < KT; ++j) {
+          if (s.row[j] < 0) continue;
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            float f[L::N];
+            L::load(f, v[j][i]);
+#pragma unroll
+            for (int u = 0; u < L::N; ++u) acc[i][u] = fmaf(s.w[j], f[u], acc[i][u]);
+          }
         }
       }
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int p = p0 + 32 * i + lane;
+        if (p < pieces) reinterpret_cast<V*>(out + t * ldo)[p] = L::store(acc[i]);
+      }
     }
-    if (live) reinterpret_cast<V*>(out + t * ldo)[piece] = L::store(acc);
   }
 }
 
-// WARPS warps per token: the token's output gradient is read once, every
-// slot's row is read once for its dot product and its gradient written.
-template <typename S, int W, int WARPS>
+// WARPS warps per token: the token's output gradient is read once per round of
+// KT slots, every slot's row once for its dot product, and its gradient written.
+template <typename S, int W, int KT, int U, int WARPS>
 __global__ void __launch_bounds__(128)
     combine_bwd_kernel(S* __restrict__ gy, long long ldgy, void* __restrict__ gw,
                        const S* __restrict__ g, long long ldg, const S* __restrict__ y,
                        long long ldy, const int32_t* __restrict__ position,
                        const void* __restrict__ w, int w_dtype, long long T, int k, long long n,
-                       long long pieces) {
+                       int pieces) {
   using L = Elems<S, W>;
   using V = typename L::V;
   constexpr int TOKENS = 4 / WARPS;  // per block
-  __shared__ float part[TOKENS][WARPS][SLOTS];
+  __shared__ float part[4][KT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int slot_t = warp / WARPS, sub = warp % WARPS;
-  const int tid = sub * 32 + lane;
+  const int sub = warp % WARPS;
   for (long long t0 = (long long)blockIdx.x * TOKENS; t0 < T; t0 += (long long)gridDim.x * TOKENS) {
-    const long long t = t0 + slot_t;
-    const bool on = t < T;
-    for (int j0 = 0; j0 < k; j0 += SLOTS) {
-      int p = 0;
-      float wt = 0.f;
-      if (on && lane < SLOTS && j0 + lane < k) {
-        p = position[t * k + j0 + lane];
-        if (p >= 0) wt = weight_at(w, w_dtype, t * k + j0 + lane);
+    const long long t = t0 + warp / WARPS;
+    if (WARPS == 1 && t >= T) break;
+    const V* gr = reinterpret_cast<const V*>(g + t * ldg);
+    for (int j0 = 0; j0 < k; j0 += KT) {
+      Slots<KT> s;
+      s.load(position, w, w_dtype, t, k, j0, n);
+      // rows of pairs without an expert, whose gradient is zero
+      int bare[KT];
+#pragma unroll
+      for (int j = 0; j < KT; ++j) {
+        bare[j] = -1;
+        if (s.row[j] < 0 && j0 + j < k && gy) {
+          const int p = position[t * k + j0 + j];
+          if (p < 0 && -1LL - p < n) bare[j] = -1 - p;
+        }
       }
-      int pj[SLOTS];
-      float wj[SLOTS], dot[SLOTS];
+      float dot[KT];
 #pragma unroll
-      for (int j = 0; j < SLOTS; ++j) {
-        pj[j] = __shfl_sync(0xffffffffu, p, j);
-        wj[j] = __shfl_sync(0xffffffffu, wt, j);
-        dot[j] = 0.f;
-      }
-      if (on) {
-        const V* gr = reinterpret_cast<const V*>(g + t * ldg);
-        for (long long c = tid; c < pieces; c += 32 * WARPS) {
-          const V gv = gr[c];
-          V v[SLOTS];
-          if (gw) {
+      for (int j = 0; j < KT; ++j) dot[j] = 0.f;
+      for (int p0 = sub * (32 * U); p0 < pieces; p0 += WARPS * (32 * U)) {
+        V gv[U], v[KT][U];
 #pragma unroll
-            for (int j = 0; j < SLOTS; ++j)
-              if (j0 + j < k && pj[j] >= 0 && pj[j] < n)
-                v[j] = reinterpret_cast<const V*>(y + pj[j] * ldy)[c];
-          }
-          float gf[L::N];
-          L::load(gf, gv);
+        for (int i = 0; i < U; ++i) {
+          const int p = p0 + 32 * i + lane;
+          gv[i] = zero_piece<V>();
+          if (p < pieces) gv[i] = gr[p];
+        }
+        if (gw) {
 #pragma unroll
-          for (int j = 0; j < SLOTS; ++j) {
-            if (j0 + j >= k) continue;
-            const long long row = pj[j] < 0 ? -1LL - pj[j] : pj[j];
-            if (row >= n) continue;
-            if (gw && pj[j] >= 0) {
-              float f[L::N];
-              L::load(f, v[j]);
+          for (int j = 0; j < KT; ++j)
 #pragma unroll
-              for (int u = 0; u < L::N; ++u) dot[j] = fmaf(gf[u], f[u], dot[j]);
+            for (int i = 0; i < U; ++i) {
+              const int p = p0 + 32 * i + lane;
+              v[j][i] = zero_piece<V>();
+              if (p < pieces && s.row[j] >= 0)
+                v[j][i] = reinterpret_cast<const V*>(y + s.row[j] * ldy)[p];
             }
-            if (gy) {
-              V o = zero_piece<V>();
-              if (pj[j] >= 0) {
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+          const int p = p0 + 32 * i + lane;
+          float gf[L::N];
+          L::load(gf, gv[i]);
+#pragma unroll
+          for (int j = 0; j < KT; ++j) {
+            if (gw) {
+              float f[L::N];
+              L::load(f, v[j][i]);
+#pragma unroll
+              for (int u = 0; u < L::N; ++u)
+                if (p < pieces && s.row[j] >= 0) dot[j] = fmaf(gf[u], f[u], dot[j]);
+            }
+            if (gy && p < pieces) {
+              if (s.row[j] >= 0) {
                 float f[L::N];
 #pragma unroll
-                for (int u = 0; u < L::N; ++u) f[u] = wj[j] * gf[u];
-                o = L::store(f);
+                for (int u = 0; u < L::N; ++u) f[u] = s.w[j] * gf[u];
+                reinterpret_cast<V*>(gy + s.row[j] * ldgy)[p] = L::store(f);
+              } else if (bare[j] >= 0) {
+                reinterpret_cast<V*>(gy + bare[j] * ldgy)[p] = zero_piece<V>();
               }
-              reinterpret_cast<V*>(gy + row * ldgy)[c] = o;
             }
           }
         }
       }
       if (gw) {
+        float mine = 0.f;  // lane j: slot j0 + j's dot product
 #pragma unroll
-        for (int j = 0; j < SLOTS; ++j) {
+        for (int j = 0; j < KT; ++j) {
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
+          if (lane == j) mine = dot[j];
         }
         if (WARPS > 1) {
-          if (lane == 0) {
+          if (lane < KT) part[warp][lane] = mine;
+          __syncthreads();
+          mine = 0.f;
+          if (lane < KT) {
 #pragma unroll
-            for (int j = 0; j < SLOTS; ++j) part[slot_t][sub][j] = dot[j];
+            for (int q = 0; q < WARPS; ++q) mine += part[warp - sub + q][lane];
           }
           __syncthreads();
         }
-        if (sub == 0 && on && lane < SLOTS && j0 + lane < k) {
-          float d = 0.f;
-          if (WARPS > 1) {
-#pragma unroll
-            for (int s = 0; s < WARPS; ++s) d += part[slot_t][s][lane];
-          } else {
-#pragma unroll
-            for (int j = 0; j < SLOTS; ++j)
-              if (j == lane) d = dot[j];
-          }
+        if (sub == 0 && lane < KT && j0 + lane < k) {
           const long long i = t * k + j0 + lane;
-          if (w_dtype == G2Q_DTYPE_F32) static_cast<float*>(gw)[i] = d;
-          else if (w_dtype == G2Q_DTYPE_BF16) static_cast<__nv_bfloat16*>(gw)[i] = of_f<__nv_bfloat16>(d);
-          else static_cast<__half*>(gw)[i] = of_f<__half>(d);
+          if (w_dtype == G2Q_DTYPE_F32) static_cast<float*>(gw)[i] = mine;
+          else if (w_dtype == G2Q_DTYPE_BF16)
+            static_cast<__nv_bfloat16*>(gw)[i] = of_f<__nv_bfloat16>(mine);
+          else static_cast<__half*>(gw)[i] = of_f<__half>(mine);
         }
-        if (WARPS > 1) __syncthreads();
       }
     }
   }
@@ -447,13 +482,52 @@ int launch_dispatch(void* out, long long ldo, const void* x, long long ldx, cons
   return G2Q_OK;
 }
 
+template <typename S, int W, int KT, int U, bool MANY>
+int launch_combine_k(void* out, long long ldo, const void* y, long long ldy,
+                     const int32_t* position, const void* w, int w_dtype, long long T, int k,
+                     int pieces, cudaStream_t st) {
+  // a row is cut into segments only where whole rows would leave warp slots idle
+  const long long most = (pieces + 32 * U - 1) / (32 * U);
+  long long segs = (148 * 32 + T - 1) / T;
+  if (segs > most) segs = most;
+  long long gx = (T + 7) / 8;
+  if (gx > 148 * 64) gx = 148 * 64;
+  combine_kernel<S, W, KT, U, MANY><<<dim3((unsigned)gx, (unsigned)segs), 256, 0, st>>>(
+      static_cast<S*>(out), ldo, static_cast<const S*>(y), ldy, position, w, w_dtype, T, k, T * k,
+      pieces);
+  G2Q_CHECK_LAUNCH();
+  return G2Q_OK;
+}
+
 template <typename S, int W>
 int launch_combine(void* out, long long ldo, const void* y, long long ldy, const int32_t* position,
                    const void* w, int w_dtype, long long T, int k, long long C, cudaStream_t st) {
-  const long long pieces = C * (long long)sizeof(S) / W, segs = (pieces + 31) / 32;
-  combine_kernel<S, W><<<warp_grid(T * segs), 256, 0, st>>>(
-      static_cast<S*>(out), ldo, static_cast<const S*>(y), ldy, position, w, w_dtype, T, k, T * k,
-      pieces, segs);
+  const long long all = C * (long long)sizeof(S) / W;
+  if (all > 0x7fffff00LL) return G2Q_ERR_UNSUPPORTED;
+  const int pieces = (int)all;
+  if (k == 1) return launch_combine_k<S, W, 1, 4, false>(out, ldo, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  if (k == 2) return launch_combine_k<S, W, 2, 4, false>(out, ldo, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  if (k <= 4) return launch_combine_k<S, W, 4, 2, false>(out, ldo, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  if (k <= SLOTS) return launch_combine_k<S, W, 8, 1, false>(out, ldo, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  return launch_combine_k<S, W, 8, 1, true>(out, ldo, y, ldy, position, w, w_dtype, T, k, pieces, st);
+}
+
+template <typename S, int W, int KT, int U>
+int launch_combine_bwd_k(void* gy, long long ldgy, void* gw, const void* g, long long ldg,
+                         const void* y, long long ldy, const int32_t* position, const void* w,
+                         int w_dtype, long long T, int k, int pieces, cudaStream_t st) {
+  // one warp per token where the rows are short or the tokens fill the machine
+  if (pieces <= 32 * U || T >= 148 * 16) {
+    long long blocks = (T + 3) / 4;
+    if (blocks > 148 * 64) blocks = 148 * 64;
+    combine_bwd_kernel<S, W, KT, U, 1><<<(unsigned)blocks, 128, 0, st>>>(
+        static_cast<S*>(gy), ldgy, gw, static_cast<const S*>(g), ldg, static_cast<const S*>(y), ldy,
+        position, w, w_dtype, T, k, T * k, pieces);
+  } else {
+    combine_bwd_kernel<S, W, KT, U, 4><<<(unsigned)T, 128, 0, st>>>(
+        static_cast<S*>(gy), ldgy, gw, static_cast<const S*>(g), ldg, static_cast<const S*>(y), ldy,
+        position, w, w_dtype, T, k, T * k, pieces);
+  }
   G2Q_CHECK_LAUNCH();
   return G2Q_OK;
 }
@@ -462,22 +536,13 @@ template <typename S, int W>
 int launch_combine_bwd(void* gy, long long ldgy, void* gw, const void* g, long long ldg,
                        const void* y, long long ldy, const int32_t* position, const void* w,
                        int w_dtype, long long T, int k, long long C, cudaStream_t st) {
-  const long long pieces = C * (long long)sizeof(S) / W;
-  // one warp per token for short rows
-  if (pieces <= 64) {
-    long long blocks = (T + 3) / 4;
-    if (blocks > 148 * 64) blocks = 148 * 64;
-    combine_bwd_kernel<S, W, 1><<<(unsigned)blocks, 128, 0, st>>>(
-        static_cast<S*>(gy), ldgy, gw, static_cast<const S*>(g), ldg, static_cast<const S*>(y), ldy,
-        position, w, w_dtype, T, k, T * k, pieces);
-  } else {
-    long long blocks = T < 148 * 64 ? T : 148 * 64;
-    combine_bwd_kernel<S, W, 4><<<(unsigned)blocks, 128, 0, st>>>(
-        static_cast<S*>(gy), ldgy, gw, static_cast<const S*>(g), ldg, static_cast<const S*>(y), ldy,
-        position, w, w_dtype, T, k, T * k, pieces);
-  }
-  G2Q_CHECK_LAUNCH();
-  return G2Q_OK;
+  const long long all = C * (long long)sizeof(S) / W;
+  if (all > 0x7fffff00LL) return G2Q_ERR_UNSUPPORTED;
+  const int pieces = (int)all;
+  if (k == 1) return launch_combine_bwd_k<S, W, 1, 4>(gy, ldgy, gw, g, ldg, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  if (k == 2) return launch_combine_bwd_k<S, W, 2, 4>(gy, ldgy, gw, g, ldg, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  if (k <= 4) return launch_combine_bwd_k<S, W, 4, 2>(gy, ldgy, gw, g, ldg, y, ldy, position, w, w_dtype, T, k, pieces, st);
+  return launch_combine_bwd_k<S, W, 8, 1>(gy, ldgy, gw, g, ldg, y, ldy, position, w, w_dtype, T, k, pieces, st);
 }
 
 bool routed_shape_ok(long long T, long long k, long long C) {
