@@ -82,7 +82,7 @@ __device__ __forceinline__ unsigned top_of(unsigned m) {
 }
 
 // round(v / scale), ties to even, of the real quotient, for a quotient whose
-// product with the rounded reciprocal lies within 1e-4 of the half-integer h
+// product with the rounded reciprocal lies within 1e-5 of the half-integer h
 // between n and its neighbour: the sign of the exactly rounded residual
 // v - h * scale decides.
 __device__ __forceinline__ int code_near_tie(float v, float scale, float n, float d) {
@@ -94,9 +94,9 @@ __device__ __forceinline__ int code_near_tie(float v, float scale, float n, floa
 }
 
 // Codes of a unit, four to a word.  The product with the rounded reciprocal is
-// within 1e-4 of the quotient (of at most 127), so its rounding is the
-// quotient's unless it lands that near a half-integer: then (one unit in some
-// hundreds) the unit's near ties are settled one by one.
+// within 127 * 2^-24 < 1e-5 of the quotient, so its rounding is the
+// quotient's unless it lands that near a half-integer: then (one unit in a
+// thousand) the unit's near ties are settled one by one.
 template <typename S>
 __device__ __forceinline__ void unit_codes(const Unit<S>& u, float scale, float inv,
                                            uint32_t (&w)[4]) {
@@ -113,7 +113,7 @@ __device__ __forceinline__ void unit_codes(const Unit<S>& u, float scale, float 
     }
     w[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
   }
-  if (far > 0.4999f) {
+  if (far > 0.49999f) {
 #pragma unroll 1
     for (int i = 0; i < 16; ++i) {
       float v = u.at(0);
@@ -121,7 +121,7 @@ __device__ __forceinline__ void unit_codes(const Unit<S>& u, float scale, float 
       for (int k = 1; k < 16; ++k)
         if (k == i) v = u.at(k);
       const float t = fmaf(v, inv, kMagic), n = t - kMagic, d = fmaf(v, inv, -n);
-      if (fabsf(d) > 0.4999f) {
+      if (fabsf(d) > 0.49999f) {
         const uint32_t code = static_cast<uint32_t>(code_near_tie(v, scale, n, d)) & 255u;
         const int sh = 8 * (i % 4);
 #pragma unroll

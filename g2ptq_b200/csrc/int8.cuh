@@ -43,34 +43,37 @@ static inline long long range_slots(const Product& p, int tile) {
   return p.offsets ? full + (p.groups < p.M ? p.groups : p.M) : full;
 }
 
-// Bounds of group g, made safe against offsets that are not ascending within
-// [0, M]: every piece lies in [0, M].
-__device__ __forceinline__ void group_bounds(const Product& p, long long g, long long* lo,
-                                             long long* hi) {
-  long long a = g == 0 ? 0 : p.offsets[g], b = g < p.groups ? (long long)p.offsets[g + 1] : p.M;
-  a = a < 0 ? 0 : (a > p.M ? p.M : a);
-  b = b < a ? a : (b > p.M ? p.M : b);
-  *lo = a;
-  *hi = b;
+// First row of group g (of group == groups: of the rows behind the last one;
+// beyond: M), for 32 neighbouring g of a warp's lanes in ascending calls with
+// *top = 0 before the first: the running maximum of the offsets within [0, M],
+// so that the groups partition [0, M] whatever the offsets hold.
+__device__ __forceinline__ long long group_start(const Product& p, long long g, long long* top) {
+  const int lane = threadIdx.x & 31;
+  long long v = 0;
+  if (g > p.groups || (!p.offsets && g > 0)) v = p.M;
+  else if (g > 0) v = p.offsets[g];
+  v = v < *top ? *top : (v > p.M ? p.M : v);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o && up > v) v = up;
+  }
+  *top = __shfl_sync(0xffffffffu, v, 31);
+  return v;
 }
 
 // The slot-th piece of `tile` rows, counted through the groups in order (one
-// warp; lane 0 writes *out).
+// warp; one lane writes *out).
 __device__ __forceinline__ void find_range(const Product& p, long long slot, int tile, Range* out) {
   const int lane = threadIdx.x & 31;
-  if (!p.offsets) {
-    if (lane == 0) {
-      const long long row0 = slot * tile, left = p.M - row0;
-      *out = Range{row0, (int)(left < tile ? left : tile), 0};
-    }
-    return;
-  }
-  long long before = 0;
-  for (long long g0 = 0; g0 <= p.groups; g0 += 32) {
+  long long before = 0, top = 0;
+  for (long long g0 = 0; g0 <= p.groups; g0 += 31) {
+    // 31 groups and the next one's start
     const long long g = g0 + lane;
-    long long lo = 0, hi = 0;
-    if (g <= p.groups) group_bounds(p, g, &lo, &hi);
-    const long long mine = (hi - lo + tile - 1) / tile;
+    long long from = top;
+    const long long lo = group_start(p, g, &from);
+    const long long hi = __shfl_down_sync(0xffffffffu, lo, 1);
+    const long long mine = lane < 31 && g <= p.groups ? (hi - lo + tile - 1) / tile : 0;
     long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -85,6 +88,7 @@ __device__ __forceinline__ void find_range(const Product& p, long long slot, int
     }
     if (__any_sync(0xffffffffu, here)) return;
     before += __shfl_sync(0xffffffffu, sum, 31);
+    top = __shfl_sync(0xffffffffu, lo, 30);
   }
   if (lane == 0) *out = Range{0, 0, 0};
 }

@@ -40,7 +40,7 @@ constexpr int STAGE_BYTES = KC * 2 * OP_BYTES;
 constexpr int STAGES = 3;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
-constexpr int STRIP_BYTES = 16 * (32 * 4 + 16);  // 16 tokens x 32 channels, padded
+constexpr int STRIP_BYTES = 16 * 32 * 2;  // 16 tokens x 32 channels of 2 bytes
 constexpr int RASTER = 8;            // row pieces walked together
 
 struct TcArgs {
@@ -58,41 +58,35 @@ struct Tile {
   int k0, k1, split;  // K range in chunks
 };
 
-// In shared memory: the first piece of each group and the groups' bounds, so
-// that every role finds its tile by a binary search.
+// In shared memory: the first piece and the first row of each group (and what
+// would follow the last), so that every role finds its tile by a binary search.
 struct Table {
   int32_t* first;  // [groups + 2]
-  int32_t* lo;     // [groups + 1]
-  int32_t* hi;
+  int32_t* lo;     // [groups + 2]
 };
 
 __device__ __forceinline__ void build_table(const Product& p, int tok, const Table& t) {
   const int lane = threadIdx.x & 31;
+  const int ends = (int)p.groups + 2;
+  long long top = 0;
+  for (int g0 = 0; g0 < ends; g0 += 32) {
+    const long long lo = group_start(p, g0 + lane, &top);
+    if (g0 + lane < ends) t.lo[g0 + lane] = (int)lo;
+  }
+  __syncwarp();
   int before = 0;
-  for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+  for (int g0 = 0; g0 < ends; g0 += 32) {
     const int g = g0 + lane;
-    long long lo = 0, hi = 0;
-    if (g <= p.groups) {
-      if (p.offsets) {
-        group_bounds(p, g, &lo, &hi);
-      } else {
-        lo = g == 0 ? 0 : p.M;
-        hi = p.M;
-      }
-      t.lo[g] = (int)lo;
-      t.hi[g] = (int)hi;
-    }
-    const int mine = ((int)(hi - lo) + tok - 1) / tok;
+    const int mine = g + 1 < ends ? (t.lo[g + 1] - t.lo[g] + tok - 1) / tok : 0;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += up;
     }
-    if (g <= p.groups) t.first[g] = before + sum - mine;
+    if (g < ends) t.first[g] = before + sum - mine;
     before += __shfl_sync(0xffffffffu, sum, 31);
   }
-  if (lane == 0) t.first[p.groups + 1] = before;
 }
 
 __device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, int w) {
@@ -116,7 +110,7 @@ __device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, int w) {
   }
   r.group = lo;
   r.row0 = t.lo[lo] + (piece - t.first[lo]) * a.tok;
-  const int left = t.hi[lo] - r.row0;
+  const int left = t.lo[lo + 1] - r.row0;
   r.rows = left < a.tok ? left : a.tok;
   r.k0 = r.split * a.per_split;
   r.k1 = r.k0 + a.per_split < a.nk ? r.k0 + a.per_split : a.nk;
@@ -156,38 +150,45 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       : "memory");
 }
 
-// Sixteen tokens (columns) of a warp's 32 channels to memory: dst points at the
-// first token's row and the strip's first channel, `n` channels and `rows`
-// tokens of it exist.  Each lane holds one channel, so the values pass through a
-// padded strip of shared memory to leave as 16-byte pieces of token rows.
-template <typename T>
-__device__ __forceinline__ void store16(T* dst, long long ld, int rows, long long n, bool vec,
-                                        uint8_t* strip, const T (&v)[16]) {
-  constexpr int PITCH = 32 * (int)sizeof(T) + 16;
-  constexpr int PER = 16 / (int)sizeof(T);  // elements per piece
-  constexpr int PIECES = 32 / PER;          // pieces per token
-  const int lane = threadIdx.x & 31;
-  if (vec) {
-#pragma unroll
-    for (int c = 0; c < 16; ++c) reinterpret_cast<T*>(strip + c * PITCH)[lane] = v[c];
-    __syncwarp();
-    const int piece = lane % PIECES;
-    T* d = dst + (lane / PIECES) * ld + piece * PER;
-    const bool in = piece * PER < n;
-#pragma unroll
-    for (int i = 0; i < 16 * PIECES / 32; ++i) {
-      const int c = i * (32 / PIECES) + lane / PIECES;
-      if (in && c < rows)
-        *reinterpret_cast<uint4*>(d + (long long)i * (32 / PIECES) * ld) =
-            *reinterpret_cast<const uint4*>(strip + c * PITCH + piece * 16);
-    }
-    __syncwarp();
-  } else {
-#pragma unroll
-    for (int c = 0; c < 16; ++c)
-      if (lane < n && c < rows) dst[c * ld + lane] = v[c];
-  }
+// 32 columns (tokens) of 16 TMEM lanes (channels) as matrix fragments: lane l
+// holds channels l / 4 and l / 4 + 8, of columns 8 j + 2 (l % 4) and the next in
+// r[4 j], r[4 j + 1] and r[4 j + 2], r[4 j + 3].  No wait.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
+
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit values, transposed: lane l gives the address of
+// row l % 8 of matrix l / 8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                  uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr),
+               "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+template <typename S>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  S v[2] = {of_f<S>(a), of_f<S>(b)};
+  uint32_t w;
+  memcpy(&w, v, 4);
+  return w;
+}
+
+// The channel scales and biases that one lane needs: one channel where lanes are
+// channels (the first entry), four in fragment order.
+struct Channels {
+  float sb[4], bias[4];
+};
 
 template <typename S>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -208,7 +209,6 @@ __global__ void __launch_bounds__(THREADS, 1)
   Table table;
   table.first = reinterpret_cast<int32_t*>(sa_s + 2 * TOK);
   table.lo = table.first + p.groups + 2;
-  table.hi = table.lo + p.groups + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
@@ -338,26 +338,40 @@ __global__ void __launch_bounds__(THREADS, 1)
       }
     }
   } else {
-    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (channels) of this CTA; the two
-    // warps of a quadrant take alternate blocks of 32 tokens
-    const int q = warp & 3, half = (warp - 2) / 4, et = threadIdx.x - 64;
+    // warp w reads TMEM lanes 32 (w % 4) .. + 31 (channels) of this CTA; the
+    // warps of a quadrant take turns at blocks of 32 tokens
+    const int q = warp & 3, part = (warp - 2) / 4, et = threadIdx.x - 64;
     const uint32_t acce_lead = mapa_shared(acce0, 0);
-    uint8_t* strip = strips + (warp - 2) * STRIP_BYTES;
     S* out = static_cast<S*>(p.out);
-    const bool vec = a.splits > 1 ? p.N % 4 == 0
-                                  : (reinterpret_cast<uintptr_t>(out) & 15) == 0 &&
-                                        p.ldo * sizeof(S) % 16 == 0 && p.N * sizeof(S) % 16 == 0;
+    // 16-bit outputs leave as 16-byte pieces of token rows, through a strip of 16
+    // tokens x 32 channels whose pieces are swizzled (piece ^ token / 2) so that
+    // neither the transposing stores nor the row reads conflict: the MMAs read
+    // their operands from the same shared memory at most of its rate, and 2-byte
+    // stores to it took 168 us where this takes YYY (65536 rows of 768 through
+    // 128 experts of 2048 channels).  32-bit values leave straight from the
+    // registers, a warp's 32 channels being 128 bytes of a token's row.
+    const bool frag = sizeof(S) == 2 && a.splits == 1 &&
+                      (reinterpret_cast<uintptr_t>(out) & 15) == 0 && p.ldo % 8 == 0 &&
+                      p.N % 8 == 0;
+    uint8_t* strip = strips + (warp - 2) * STRIP_BYTES;
+    const uint32_t st_row = smem_u32(strip) + (lane % 8) * 64 + (((lane / 8) ^ (lane % 8 / 2)) * 16);
+    const uint8_t* ld_row = strip + (lane / 4) * 64 + (((lane % 4) ^ (lane / 4 / 2 % 4)) * 16);
     Tile t, next;
-    float sa_next = 0.f, sb_next = 0.f, bias_next = 0.f;
+    float sa_next = 0.f;
+    Channels ch_next;
     // a tile's scales are loaded one tile ahead; zeros where there is no such
     // row or channel, and for rows behind the last group
     auto fetch = [&](int w) {
       next = decode(a, table, w);
       const bool zero = next.group == p.groups;
-      const int n = next.ch0 + 128 * (int)rank + q * 32 + lane;
       sa_next = !zero && et < next.rows ? p.sa[next.row0 + et] : 0.f;
-      sb_next = !zero && n < p.N ? p.sb[(long long)next.group * p.N + n] : 0.f;
-      bias_next = p.bias && n < p.N ? p.bias[n] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (u > 0 && !frag) break;
+        const int n = next.ch0 + 128 * (int)rank + q * 32 + (frag ? lane / 4 + 8 * u : lane);
+        ch_next.sb[u] = !zero && n < p.N ? p.sb[(long long)next.group * p.N + n] : 0.f;
+        ch_next.bias[u] = p.bias && n < p.N ? p.bias[n] : 0.f;
+      }
     };
     int tc = 0, turn = 0, w = blockIdx.x >> 1;
     bool ok = true;
@@ -365,9 +379,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (w < total) fetch(w);
     for (; w < total; w += step, ++turn) {
       t = next;
-      const float sb = sb_next, bias = bias_next;
+      const Channels ch = ch_next;
       float* sa = sa_s + (turn & 1) * TOK;
-      sa[et] = sa_next;
+      if (et < TOK) sa[et] = sa_next;
       asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
       if (w + step < total) fetch(w + step);
       const bool zero = t.group == p.groups;
@@ -382,37 +396,66 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t base = tmem + (uint32_t)(buf * TOK) + ((uint32_t)(q * 32) << 16);
       const long long n0 = t.ch0 + 128 * (long long)rank + q * 32;
       const long long n = p.N - n0;  // channels of the strip (may be none)
-      for (int c0 = 32 * half; c0 < t.rows; c0 += 64) {
-        uint32_t r[32];
-        if (zero) {
+      for (int c0 = 32 * part; c0 < t.rows; c0 += 8 * EPI_WARPS) {
+        const long long row = t.row0 + c0;
+        const int rows = t.rows - c0;
+        if (frag) {
+          uint32_t r[2][16];
+          if (zero) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) r[c] = 0;
-        } else {
-          tmem_ld32(base + (uint32_t)c0, r);
-        }
-        if (!ok) continue;
-#pragma unroll
-        for (int h = 0; h < 32; h += 16) {
-          const long long row = t.row0 + c0 + h;
-          const int rows = t.rows - c0 - h;
-          if (rows <= 0) break;
-          if (a.splits > 1) {
-            int v[16];
-#pragma unroll
-            for (int c = 0; c < 16; ++c) v[c] = (int)r[h + c];
-            store16<int>(a.part + ((long long)t.split * p.M + row) * p.N + n0, p.N, rows, n, vec,
-                         strip, v);
+            for (int u = 0; u < 16; ++u) r[0][u] = r[1][u] = 0;
           } else {
-            S v[16];
+            tmem_ld_16x256b_x4(base + (uint32_t)c0, r[0]);
+            tmem_ld_16x256b_x4(base + (uint32_t)c0 + (16u << 16), r[1]);
+            tmem_wait_ld();
+          }
+          if (!ok) continue;
 #pragma unroll
-            for (int c4 = 0; c4 < 16; c4 += 4) {
-              const float4 s4 = *reinterpret_cast<const float4*>(sa + c0 + h + c4);
-              v[c4] = of_f<S>(scaled((int)r[h + c4], s4.x, sb, bias));
-              v[c4 + 1] = of_f<S>(scaled((int)r[h + c4 + 1], s4.y, sb, bias));
-              v[c4 + 2] = of_f<S>(scaled((int)r[h + c4 + 2], s4.z, sb, bias));
-              v[c4 + 3] = of_f<S>(scaled((int)r[h + c4 + 3], s4.w, sb, bias));
+          for (int h = 0; h < 2; ++h) {  // 16 tokens
+            if (16 * h >= rows) break;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {  // 8 of them
+              const float2 s2 =
+                  *reinterpret_cast<const float2*>(sa + c0 + 16 * h + 8 * j + 2 * (lane % 4));
+              uint32_t m[4];
+#pragma unroll
+              for (int u = 0; u < 4; ++u) {
+                const uint32_t* v = &r[u / 2][8 * h + 4 * j + 2 * (u % 2)];
+                m[u] = pack2<S>(scaled((int)v[0], s2.x, ch.sb[u], ch.bias[u]),
+                                scaled((int)v[1], s2.y, ch.sb[u], ch.bias[u]));
+              }
+              stmatrix_x4_trans(st_row + 8 * j * 64, m[0], m[1], m[2], m[3]);
             }
-            store16<S>(out + row * p.ldo + n0, p.ldo, rows, n, vec, strip, v);
+            __syncwarp();
+            S* dst = out + (row + 16 * h + lane / 4) * p.ldo + n0 + 8 * (lane % 4);
+            const bool in = 8 * (lane % 4) < n;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)  // 8 tokens
+              if (in && 16 * h + 8 * i + lane / 4 < rows)
+                *reinterpret_cast<uint4*>(dst + (long long)i * 8 * p.ldo) =
+                    *reinterpret_cast<const uint4*>(ld_row + i * 8 * 64);
+            __syncwarp();
+          }
+        } else {
+          uint32_t r[32];
+          if (zero) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) r[c] = 0;
+          } else {
+            tmem_ld32(base + (uint32_t)c0, r);
+          }
+          if (!ok || lane >= n) continue;
+          if (a.splits > 1) {
+            int32_t* dst = a.part + ((long long)t.split * p.M + row) * p.N + n0 + lane;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c < rows) dst[c * p.N] = (int)r[c];
+          } else {
+            S* dst = out + row * p.ldo + n0 + lane;
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (c < rows)
+                dst[c * p.ldo] = of_f<S>(scaled((int)r[c], sa[c0 + c], ch.sb[0], ch.bias[0]));
           }
         }
       }
@@ -544,7 +587,7 @@ static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, 
                      cudaStream_t st) {
   const int smem = STAGES * STAGE_BYTES + 1024 + 128 + EPI_WARPS * STRIP_BYTES +
                    2 * TOK * (int)sizeof(float) +
-                   (int)(3 * a.p.groups + 4) * (int)sizeof(int32_t);
+                   (int)(2 * a.p.groups + 4) * (int)sizeof(int32_t);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return G2Q_ERR_CUDA;
   static int attr_done[64] = {0};
