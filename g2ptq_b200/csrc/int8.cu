@@ -7,6 +7,8 @@
 // The sums are exact in 32-bit integers (|q w| <= 128 * 128, C <= 131071); the
 // only roundings are the conversion of the sum to fp32, the two scalings, the
 // bias and the output type.
+#include <type_traits>
+
 #include "int8.cuh"
 #include "rows.cuh"
 #include "tc_ptx.cuh"
@@ -29,31 +31,31 @@ struct Unit {
   static constexpr int W = 16 * (int)sizeof(S) / 4;  // 32-bit words
   uint32_t raw[W];
 
-  __device__ __forceinline__ void load(const S* p, int have, bool vec) {
-    if (vec && have >= 16) {
+  __device__ __forceinline__ void load(const S* p) {
 #pragma unroll
-      for (int i = 0; i < W / 4; ++i) {
-        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-        raw[4 * i] = v.x;
-        raw[4 * i + 1] = v.y;
-        raw[4 * i + 2] = v.z;
-        raw[4 * i + 3] = v.w;
-      }
-    } else {
-      S e[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = i < have ? p[i] : of_f<S>(0.f);
-      memcpy(raw, e, sizeof(raw));
+    for (int i = 0; i < W / 4; ++i) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+      raw[4 * i] = v.x;
+      raw[4 * i + 1] = v.y;
+      raw[4 * i + 2] = v.z;
+      raw[4 * i + 3] = v.w;
     }
+  }
+  __device__ __forceinline__ void load_part(const S* p, int have) {
+    S e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) e[i] = i < have ? p[i] : of_f<S>(0.f);
+    memcpy(raw, e, sizeof(raw));
   }
   __device__ __forceinline__ float at(int i) const {
     if constexpr (sizeof(S) == 4) {
       return __uint_as_float(raw[i]);
+    } else if constexpr (std::is_same_v<S, __nv_bfloat16>) {
+      return __uint_as_float(i % 2 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
     } else {
-      const uint16_t h = (uint16_t)(raw[i / 2] >> (16 * (i % 2)));
-      S v;
-      memcpy(&v, &h, 2);
-      return to_f<S>(v);
+      __half2 h;
+      memcpy(&h, &raw[i / 2], 4);
+      return i % 2 ? __high2float(h) : __low2float(h);
     }
   }
   // the largest magnitude: the bits of a non-negative number order like an
@@ -68,6 +70,12 @@ struct Unit {
   }
 };
 
+// The larger of two such values
+template <typename S>
+__device__ __forceinline__ unsigned max_bits(unsigned a, unsigned b) {
+  return sizeof(S) == 4 ? max(a, b) : __vmaxu2(a, b);
+}
+
 // fp32 bits of the magnitude that top_bits collected
 template <typename S>
 __device__ __forceinline__ unsigned top_of(unsigned m) {
@@ -81,62 +89,65 @@ __device__ __forceinline__ unsigned top_of(unsigned m) {
   }
 }
 
-// round(v / scale), ties to even, of the real quotient, for a quotient whose
-// product with the rounded reciprocal lies within 1e-5 of the half-integer h
-// between n and its neighbour: the sign of the exactly rounded residual
-// v - h * scale decides.
-__device__ __forceinline__ int code_near_tie(float v, float scale, float n, float d) {
-  const float h = n + copysignf(0.5f, d);
-  const float res = fmaf(-h, scale, v);
-  const float lo = h - 0.5f, hi = h + 0.5f;
+// What a row's codes are made with: the scale, and factors just below and above
+// its reciprocal, so that the real quotient v / scale lies between the products
+// v * below and v * above.
+struct RowScale {
+  float scale, below, above;
+};
+
+// The real quotient's rounding, ties to even, where it lies next to the
+// half-integer between the neighbouring integers a and b: the sign of the exactly
+// rounded residual v - h * scale tells on which side.
+__device__ __forceinline__ int settle(float v, float scale, float a, float b) {
+  const float lo = fminf(a, b), hi = fmaxf(a, b);
+  const float res = fmaf(-(lo + 0.5f), scale, v);
   const float even = (static_cast<int>(lo) & 1) ? hi : lo;
   return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
 }
 
-// Codes of a unit, four to a word.  The product with the rounded reciprocal is
-// within 127 * 2^-24 < 1e-5 of the quotient, so its rounding is the
-// quotient's unless it lands that near a half-integer: then (one unit in a
-// thousand) the unit's near ties are settled one by one.
+// Codes of a unit, four to a word: round(v / scale) of the real quotient.  Where
+// its two bounds round to the same integer the quotient does too; the others are
+// settled one by one.  They are not that rare: in 16-bit inputs many values are
+// exactly half of the row's largest one, whose quotient is 63.5 but for the
+// scale's own rounding.
 template <typename S>
-__device__ __forceinline__ void unit_codes(const Unit<S>& u, float scale, float inv,
-                                           uint32_t (&w)[4]) {
+__device__ __forceinline__ void unit_codes(const Unit<S>& u, const RowScale& rs, uint32_t (&w)[4]) {
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the integer's
-  float far = 0.f;
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
-    uint32_t b[4];
+    uint32_t a[4], b[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float v = u.at(4 * g + i), t = fmaf(v, inv, kMagic), n = t - kMagic;
-      far = fmaxf(far, fabsf(fmaf(v, inv, -n)));
-      b[i] = __float_as_uint(t);
+      const float v = u.at(4 * g + i);
+      a[i] = __float_as_uint(fmaf(v, rs.below, kMagic));
+      b[i] = __float_as_uint(fmaf(v, rs.above, kMagic));
     }
-    w[g] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-  }
-  if (far > 0.49999f) {
-#pragma unroll 1
-    for (int i = 0; i < 16; ++i) {
-      float v = u.at(0);
-#pragma unroll
-      for (int k = 1; k < 16; ++k)
-        if (k == i) v = u.at(k);
-      const float t = fmaf(v, inv, kMagic), n = t - kMagic, d = fmaf(v, inv, -n);
-      if (fabsf(d) > 0.49999f) {
-        const uint32_t code = static_cast<uint32_t>(code_near_tie(v, scale, n, d)) & 255u;
-        const int sh = 8 * (i % 4);
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          if (g == i / 4) w[g] = (w[g] & ~(255u << sh)) | code << sh;
-      }
+    const uint32_t wa =
+        __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
+    const uint32_t wb =
+        __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+    w[g] = wa;
+    uint32_t differ = wa ^ wb;
+    while (differ) {
+      const int i = (__ffs(differ) - 1) / 8;
+      const float v01 = i & 1 ? u.at(4 * g + 1) : u.at(4 * g);
+      const float v23 = i & 1 ? u.at(4 * g + 3) : u.at(4 * g + 2);
+      const float v = i & 2 ? v23 : v01;
+      const int code = settle(v, rs.scale, fmaf(v, rs.below, kMagic) - kMagic,
+                              fmaf(v, rs.above, kMagic) - kMagic);
+      const uint32_t mask = 255u << (8 * i);
+      w[g] = (w[g] & ~mask) | ((static_cast<uint32_t>(code) << (8 * i)) & mask);
+      differ &= ~mask;
     }
   }
 }
 
 template <typename S>
 __device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int have, bool vec,
-                                            float scale, float inv, bool finite) {
+                                            const RowScale& rs, bool finite) {
   uint32_t w[4] = {0, 0, 0, 0};
-  if (finite) unit_codes<S>(u, scale, inv, w);
+  if (finite) unit_codes<S>(u, rs, w);
   if (vec && have >= 16) {
     *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   } else {
@@ -146,22 +157,27 @@ __device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int h
   }
 }
 
-// Scale of a row from its largest magnitude's bits, and the reciprocal; false
-// where a value is not finite, which makes the whole row NaN (codes zero).
-__device__ __forceinline__ bool row_scale(unsigned top, float* scale, float* inv) {
-  *scale = __fdiv_rn(__uint_as_float(top), 127.f);
-  if (*scale < 1.17549435e-38f) *scale = 1.f;  // zeros (and values below the normal range)
-  *inv = __frcp_rn(*scale);
+// Scale of a row from its largest magnitude's bits; false where a value is not
+// finite, which makes the whole row NaN (codes zero).  The reciprocal is within
+// 2^-24 of 1 / scale, so 2^-22 either way brackets it.
+__device__ __forceinline__ bool row_scale(unsigned top, RowScale* rs) {
+  float scale = __fdiv_rn(__uint_as_float(top), 127.f);
+  if (scale < 1.17549435e-38f) scale = 1.f;  // zeros (and values below the normal range)
+  const float inv = __frcp_rn(scale);
+  rs->scale = scale;
+  rs->below = __fmul_rd(inv, 1.f - 2.3841858e-7f);
+  rs->above = __fmul_ru(inv, 1.f + 2.3841858e-7f);
   return top < kInfBits;
 }
 
 // G threads per row, UNITS units of 16 elements per thread kept in registers
-// between the maximum and the codes (one read of x); what a longer row has
-// beyond UNITS * G units is read a second time.
+// between the maximum and the codes (one read of x).  What is left of a row --
+// the units beyond UNITS * G, a part of a unit at its end, all of a row that is
+// not 16-byte aligned -- goes element by element and is read a second time.
 template <typename S, int G, int UNITS>
 __global__ void __launch_bounds__(G > 128 ? G : 128)
     quantize_kernel(int8_t* __restrict__ codes, long long ldq, float* __restrict__ scale_out,
-                    const S* __restrict__ x, long long ldx, long long T, long long C, bool xvec,
+                    const S* __restrict__ x, long long ldx, long long T, int C, bool xvec,
                     bool qvec) {
   constexpr int BLOCK = G > 128 ? G : 128;
   constexpr int PER = BLOCK / G;  // rows per block
@@ -170,28 +186,23 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
   const long long t = blockIdx.x * (long long)PER + threadIdx.x / G;
   const bool live = t < T;
   const S* row = x + (live ? t : 0) * ldx;
-  const long long units = (C + 15) / 16;
+  int whole = xvec && live ? C / 16 : 0;  // units that the unrolled loops take
+  whole = whole < UNITS * G ? whole : UNITS * G;
+  const int units = live ? (C + 15) / 16 : 0;
 
   Unit<S> u[UNITS];
+#pragma unroll
+  for (int k = 0; k < UNITS; ++k)
+    if (tid + k * G < whole) u[k].load(row + 16 * (tid + k * G));
   unsigned top = 0;
-  if (live) {
 #pragma unroll
-    for (int k = 0; k < UNITS; ++k) {
-      const long long i = tid + (long long)k * G;
-      if (i < units) {
-        const long long left = C - 16 * i;
-        u[k].load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < UNITS; ++k)
-      if (tid + (long long)k * G < units) top = max(top, top_of<S>(u[k].top_bits()));
-    for (long long i = tid + (long long)UNITS * G; i < units; i += G) {
-      const long long left = C - 16 * i;
-      Unit<S> v;
-      v.load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
-      top = max(top, top_of<S>(v.top_bits()));
-    }
+  for (int k = 0; k < UNITS; ++k)
+    if (tid + k * G < whole) top = max_bits<S>(top, u[k].top_bits());
+  top = top_of<S>(top);
+  for (int i = whole + tid; i < units; i += G) {
+    Unit<S> v;
+    v.load_part(row + 16LL * i, C - 16 * i);
+    top = max(top, top_of<S>(v.top_bits()));
   }
   top = __reduce_max_sync(0xffffffffu, top);
   if constexpr (G > 32) {
@@ -203,23 +214,18 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
     for (int w = 0; w < G / 32; ++w) top = max(top, warp_top[w0 + w]);
   }
   if (!live) return;
-  float scale, inv;
-  const bool finite = row_scale(top, &scale, &inv);
-  if (tid == 0) scale_out[t] = finite ? scale : __uint_as_float(0x7fc00000u);
+  RowScale rs;
+  const bool finite = row_scale(top, &rs);
+  if (tid == 0) scale_out[t] = finite ? rs.scale : __uint_as_float(0x7fc00000u);
   int8_t* qrow = codes + t * ldq;
 #pragma unroll
-  for (int k = 0; k < UNITS; ++k) {
-    const long long i = tid + (long long)k * G;
-    if (i < units) {
-      const long long left = C - 16 * i;
-      store_codes<S>(qrow + 16 * i, u[k], left < 16 ? (int)left : 16, qvec, scale, inv, finite);
-    }
-  }
-  for (long long i = tid + (long long)UNITS * G; i < units; i += G) {
-    const long long left = C - 16 * i;
+  for (int k = 0; k < UNITS; ++k)
+    if (tid + k * G < whole)
+      store_codes<S>(qrow + 16 * (tid + k * G), u[k], 16, qvec, rs, finite);
+  for (int i = whole + tid; i < units; i += G) {
     Unit<S> v;
-    v.load(row + 16 * i, left < 16 ? (int)left : 16, xvec);
-    store_codes<S>(qrow + 16 * i, v, left < 16 ? (int)left : 16, qvec, scale, inv, finite);
+    v.load_part(row + 16LL * i, C - 16 * i);
+    store_codes<S>(qrow + 16LL * i, v, C - 16 * i, qvec, rs, finite);
   }
 }
 
@@ -228,11 +234,11 @@ static int launch_quantize(int8_t* codes, long long ldq, float* scale, const S* 
                            long long T, long long C, cudaStream_t st) {
   constexpr int BLOCK = G > 128 ? G : 128;
   const long long blocks = (T + BLOCK / G - 1) / (BLOCK / G);
-  if (blocks > 0x7fffffffLL) return G2Q_ERR_INVALID_ARG;
+  if (blocks > 0x7fffffffLL || C > 0x7fffff00LL) return G2Q_ERR_UNSUPPORTED;
   const bool xvec = rows::aligned(x, 16) && (T <= 1 || (ldx * (long long)sizeof(S)) % 16 == 0);
   const bool qvec = rows::aligned(codes, 16) && (T <= 1 || ldq % 16 == 0);
   quantize_kernel<S, G, UNITS><<<(unsigned)blocks, BLOCK, 0, st>>>(codes, ldq, scale, x, ldx, T,
-                                                                   C, xvec, qvec);
+                                                                   (int)C, xvec, qvec);
   G2Q_CHECK_LAUNCH();
   return G2Q_OK;
 }
@@ -241,12 +247,16 @@ template <typename S>
 static int quantize_rows(int8_t* codes, long long ldq, float* scale, const void* x, long long ldx,
                          long long T, long long C, cudaStream_t st) {
   const S* xs = static_cast<const S*>(x);
-  // One warp per row while a row is at most two units per lane, four warps up
-  // to 8192 columns; sixteen warps for longer rows and where few rows would
-  // leave most SMs idle.
-  if (C > 8192 || T < 2 * 148) return launch_quantize<S, 512, 2>(codes, ldq, scale, xs, ldx, T, C, st);
-  if (C > 1024) return launch_quantize<S, 128, 4>(codes, ldq, scale, xs, ldx, T, C, st);
-  return launch_quantize<S, 32, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+  // Few rows: sixteen warps each, so that more SMs and more loads are at work.
+  if (T < 2 * 148) return launch_quantize<S, 512, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+  // Else as few warps per row as its elements in registers allow (128 or 64 bytes
+  // of them per thread): the row's reduction and division serve the most elements.
+  constexpr int U = sizeof(S) == 2 ? 4 : 2;
+  if (C <= 1024) return launch_quantize<S, 32, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C <= 1024 * U) return launch_quantize<S, 64, U>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C <= 2048 * U) return launch_quantize<S, 128, U>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C <= 4096 * U) return launch_quantize<S, 256, U>(codes, ldq, scale, xs, ldx, T, C, st);
+  return launch_quantize<S, 512, U>(codes, ldq, scale, xs, ldx, T, C, st);
 }
 
 int quantize_tokens(int8_t* codes, long long ldq, float* scale, const void* x, int dtype,

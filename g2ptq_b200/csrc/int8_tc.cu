@@ -41,7 +41,9 @@ constexpr int STAGES = 3;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STRIP_BYTES = 16 * 32 * 2;  // 16 tokens x 32 channels of 2 bytes
-constexpr int RASTER = 8;            // row pieces walked together
+constexpr int RASTER = 8;            // row pieces walked together (4 and 16 measured the same)
+constexpr int BAR_BYTES = 128;       // barriers, TMEM address, abort flag
+static_assert((2 * STAGES + 5) * 8 + 8 <= BAR_BYTES, "barrier area");
 
 struct TcArgs {
   Product p;
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  uint8_t* strips = smem + STAGES * STAGE_BYTES + 128;  // [EPI_WARPS][STRIP_BYTES]
+  uint8_t* strips = smem + STAGES * STAGE_BYTES + BAR_BYTES;  // [EPI_WARPS][STRIP_BYTES]
   float* sa_s = reinterpret_cast<float*>(strips + EPI_WARPS * STRIP_BYTES);  // [2][TOK]
   Table table;
   table.first = reinterpret_cast<int32_t*>(sa_s + 2 * TOK);
@@ -585,7 +587,7 @@ size_t tc_workspace_bytes(const Product& p) {
 template <typename S>
 static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, bool overlap,
                      cudaStream_t st) {
-  const int smem = STAGES * STAGE_BYTES + 1024 + 128 + EPI_WARPS * STRIP_BYTES +
+  const int smem = STAGES * STAGE_BYTES + 1024 + BAR_BYTES + EPI_WARPS * STRIP_BYTES +
                    2 * TOK * (int)sizeof(float) +
                    (int)(2 * a.p.groups + 4) * (int)sizeof(int32_t);
   int dev = 0;
