@@ -7,168 +7,18 @@
 // The sums are exact in 32-bit integers (|q w| <= 128 * 128, C <= 131071); the
 // only roundings are the conversion of the sum to fp32, the two scalings, the
 // bias and the output type.
-#include <type_traits>
-
 #include "int8.cuh"
-#include "rows.cuh"
+#include "int8_quant.cuh"
 #include "tc_ptx.cuh"
 
 namespace g2q {
 namespace i8 {
 
 using rows::of_f;
-using rows::to_f;
 
 // ---------------------------------------------------------------------------
 // quantization of token rows
 // ---------------------------------------------------------------------------
-
-constexpr unsigned kInfBits = 0x7f800000u;
-
-// Sixteen consecutive elements of a row, raw; missing ones (beyond `have`) are zero.
-template <typename S>
-struct Unit {
-  static constexpr int W = 16 * (int)sizeof(S) / 4;  // 32-bit words
-  uint32_t raw[W];
-
-  __device__ __forceinline__ void load(const S* p) {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
-      raw[4 * i] = v.x;
-      raw[4 * i + 1] = v.y;
-      raw[4 * i + 2] = v.z;
-      raw[4 * i + 3] = v.w;
-    }
-  }
-  __device__ __forceinline__ void load_part(const S* p, int have) {
-    S e[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) e[i] = i < have ? p[i] : of_f<S>(0.f);
-    memcpy(raw, e, sizeof(raw));
-  }
-  __device__ __forceinline__ float at(int i) const {
-    if constexpr (sizeof(S) == 4) {
-      return __uint_as_float(raw[i]);
-    } else if constexpr (std::is_same_v<S, __nv_bfloat16>) {
-      return __uint_as_float(i % 2 ? raw[i / 2] & 0xffff0000u : raw[i / 2] << 16);
-    } else {
-      __half2 h;
-      memcpy(&h, &raw[i / 2], 4);
-      return i % 2 ? __high2float(h) : __low2float(h);
-    }
-  }
-  // the largest magnitude: the bits of a non-negative number order like an
-  // unsigned integer, infinities and NaN at the top.  16-bit types: the two
-  // halves of a word side by side, merged by top_of.
-  __device__ __forceinline__ unsigned top_bits() const {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-      m = sizeof(S) == 4 ? max(m, raw[i] & 0x7fffffffu) : __vmaxu2(m, raw[i] & 0x7fff7fffu);
-    return m;
-  }
-};
-
-// The larger of two such values
-template <typename S>
-__device__ __forceinline__ unsigned max_bits(unsigned a, unsigned b) {
-  return sizeof(S) == 4 ? max(a, b) : __vmaxu2(a, b);
-}
-
-// fp32 bits of the magnitude that top_bits collected
-template <typename S>
-__device__ __forceinline__ unsigned top_of(unsigned m) {
-  if constexpr (sizeof(S) == 4) {
-    return m;
-  } else {
-    const uint16_t h = (uint16_t)max(m & 0xffffu, m >> 16);
-    S v;
-    memcpy(&v, &h, 2);
-    return __float_as_uint(to_f<S>(v));
-  }
-}
-
-// What a row's codes are made with: the scale, and factors just below and above
-// its reciprocal, so that the real quotient v / scale lies between the products
-// v * below and v * above.
-struct RowScale {
-  float scale, below, above;
-};
-
-// The real quotient's rounding, ties to even, where it lies next to the
-// half-integer between the neighbouring integers a and b: the sign of the exactly
-// rounded residual v - h * scale tells on which side.
-__device__ __forceinline__ int settle(float v, float scale, float a, float b) {
-  const float lo = fminf(a, b), hi = fmaxf(a, b);
-  const float res = fmaf(-(lo + 0.5f), scale, v);
-  const float even = (static_cast<int>(lo) & 1) ? hi : lo;
-  return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
-}
-
-// Codes of a unit, four to a word: round(v / scale) of the real quotient.  Where
-// its two bounds round to the same integer the quotient does too; the others are
-// settled one by one.  They are not that rare: in 16-bit inputs many values are
-// exactly half of the row's largest one, whose quotient is 63.5 but for the
-// scale's own rounding.
-template <typename S>
-__device__ __forceinline__ void unit_codes(const Unit<S>& u, const RowScale& rs, uint32_t (&w)[4]) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the integer's
-#pragma unroll
-  for (int g = 0; g < 4; ++g) {
-    uint32_t a[4], b[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = u.at(4 * g + i);
-      a[i] = __float_as_uint(fmaf(v, rs.below, kMagic));
-      b[i] = __float_as_uint(fmaf(v, rs.above, kMagic));
-    }
-    const uint32_t wa =
-        __byte_perm(__byte_perm(a[0], a[1], 0x0040), __byte_perm(a[2], a[3], 0x0040), 0x5410);
-    const uint32_t wb =
-        __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
-    w[g] = wa;
-    uint32_t differ = wa ^ wb;
-    while (differ) {
-      const int i = (__ffs(differ) - 1) / 8;
-      const float v01 = i & 1 ? u.at(4 * g + 1) : u.at(4 * g);
-      const float v23 = i & 1 ? u.at(4 * g + 3) : u.at(4 * g + 2);
-      const float v = i & 2 ? v23 : v01;
-      const int code = settle(v, rs.scale, fmaf(v, rs.below, kMagic) - kMagic,
-                              fmaf(v, rs.above, kMagic) - kMagic);
-      const uint32_t mask = 255u << (8 * i);
-      w[g] = (w[g] & ~mask) | ((static_cast<uint32_t>(code) << (8 * i)) & mask);
-      differ &= ~mask;
-    }
-  }
-}
-
-template <typename S>
-__device__ __forceinline__ void store_codes(int8_t* dst, const Unit<S>& u, int have, bool vec,
-                                            const RowScale& rs, bool finite) {
-  uint32_t w[4] = {0, 0, 0, 0};
-  if (finite) unit_codes<S>(u, rs, w);
-  if (vec && have >= 16) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (i < have) dst[i] = static_cast<int8_t>(w[i / 4] >> (8 * (i % 4)));
-  }
-}
-
-// Scale of a row from its largest magnitude's bits; false where a value is not
-// finite, which makes the whole row NaN (codes zero).  The reciprocal is within
-// 2^-24 of 1 / scale, so 2^-22 either way brackets it.
-__device__ __forceinline__ bool row_scale(unsigned top, RowScale* rs) {
-  float scale = __fdiv_rn(__uint_as_float(top), 127.f);
-  if (scale < 1.17549435e-38f) scale = 1.f;  // zeros (and values below the normal range)
-  const float inv = __frcp_rn(scale);
-  rs->scale = scale;
-  rs->below = __fmul_rd(inv, 1.f - 2.3841858e-7f);
-  rs->above = __fmul_ru(inv, 1.f + 2.3841858e-7f);
-  return top < kInfBits;
-}
 
 // G threads per row, UNITS units of 16 elements per thread kept in registers
 // between the maximum and the codes (one read of x).  What is left of a row --
@@ -359,7 +209,13 @@ static int simt_product(const Product& p, cudaStream_t st) {
 
 static int product(const Product& p, void* workspace, size_t workspace_bytes, bool overlap,
                    cudaStream_t st) {
+  if (stream_takes(p)) return stream_product(p, overlap, st);
   return tc_takes(p) ? tc_product(p, workspace, workspace_bytes, overlap, st) : simt_product(p, st);
+}
+
+// Workspace of a product whose operands are aligned.
+static size_t product_workspace(const Product& p) {
+  return stream_takes(p) ? 0 : tc_workspace_bytes(p);
 }
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
@@ -367,7 +223,7 @@ static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 // Workspace of a linear: the tokens' codes, their scales, the product's own.
 static size_t linear_workspace(const Product& p) {
   const size_t M = (size_t)p.M, ld = (size_t)((p.K + 15) / 16 * 16);
-  return up256(M * ld) + up256(M * sizeof(float)) + tc_workspace_bytes(p);
+  return up256(M * ld) + up256(M * sizeof(float)) + product_workspace(p);
 }
 
 static int check(const Product& p) {
@@ -405,7 +261,7 @@ extern "C" size_t g2q_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t 
   p.M = M;
   p.N = N;
   p.K = K;
-  return i8::tc_workspace_bytes(p);
+  return i8::product_workspace(p);
 }
 
 extern "C" int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
@@ -465,6 +321,8 @@ extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void
   if (M == 0) return G2Q_OK;
   if (!x || !rows::aligned(workspace, 16) || workspace_bytes < i8::linear_workspace(p))
     return G2Q_ERR_INVALID_ARG;
+  if (i8::stream_quantizes(p))
+    return i8::stream_linear(p, x, x_dtype, ldx, (cudaStream_t)stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t code_bytes = i8::up256((size_t)M * (size_t)ld);
   const size_t scale_bytes = i8::up256((size_t)M * sizeof(float));

@@ -1,0 +1,239 @@
+// The 8-bit product for a handful of tokens: the weight streams through once and
+// its bytes are all the work, so what counts is loads in flight and a short way
+// from launch to result.  The tensor-core tiles (int8_tc.cu) spend several
+// microseconds on TMEM, clusters, the ring and a second kernel for K ranges.
+//
+// A CTA of eight warps takes 16 * RG channels; the warps of one 16-channel group
+// share K in turns of 64 bytes.  A lane loads 16 bytes of channels g and g + 8
+// (g = lane / 4) and 16 bytes of token g, and multiplies them with two
+// mma.sync.m16n8k32 (int8): the order of K inside a step is free as long as both
+// operands use the same, so 16 consecutive bytes serve as the four words that a
+// lane owes two steps.  The warps' integer sums meet in shared memory.
+//
+// With few enough tokens the kernel quantizes them itself (FUSED): every CTA
+// makes the codes of all tokens in shared memory, behind its first weight loads.
+#include "int8.cuh"
+#include "int8_quant.cuh"
+#include "tc_ptx.cuh"
+
+namespace g2q {
+namespace i8 {
+
+using rows::of_f;
+
+constexpr int SW = 8;       // warps per CTA
+constexpr int STEP = 64;    // bytes of K per warp and step
+constexpr int DEPTH = 4;    // steps whose loads are in flight together
+
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Bytes k .. k + 15 of a row of K bytes, missing ones zero.
+__device__ __forceinline__ uint4 load16(const int8_t* row, long long k, long long K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (k < K) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k + i < K) w[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+struct Input {  // the tokens before quantization (FUSED)
+  const void* x;
+  long long ldx;
+  bool vec;
+};
+
+// MG groups of eight tokens at a time.
+template <typename S, typename X, int RG, int MG, bool FUSED>
+__global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const Input in) {
+  constexpr int KS = SW / RG, TOKENS = 8 * MG, CHANNELS = 16 * RG;
+  extern __shared__ uint4 dyn[];  // FUSED: codes [M][pitch]
+  __shared__ int red[KS][CHANNELS][TOKENS + 1];
+  __shared__ float sa_s[TOKENS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rg = warp % RG, ks = warp / RG, g = lane / 4, t4 = lane % 4;
+  const long long group = p.offsets ? blockIdx.y : 0;
+  const long long n0 = (long long)blockIdx.x * CHANNELS;
+  long long lo = 0, hi = p.M;
+  if (p.offsets) {
+    group_bounds(p, group, &lo, &hi);
+    // the grid ends after the kernel before it even if no CTA has rows
+    if (blockIdx.x == 0 && blockIdx.y == 0) tc::wait_predecessor();
+    if (lo == hi) return;
+  }
+  S* out = static_cast<S*>(p.out);
+  if (group == p.groups) {  // rows behind the last group
+    for (long long i = threadIdx.x; i < (hi - lo) * CHANNELS; i += 32 * SW) {
+      const long long n = n0 + i % CHANNELS;
+      if (n < p.N) out[(lo + i / CHANNELS) * p.ldo + n] = of_f<S>(0.f);
+    }
+    return;
+  }
+  const int8_t* b = p.b + group * p.b_gs;
+  const long long c0 = n0 + 16 * rg + g;
+  // channels that do not exist read the last one's bytes; their sums go nowhere
+  const int8_t* w0 = b + (c0 < p.N ? c0 : p.N - 1) * p.ldb;
+  const int8_t* w1 = b + (c0 + 8 < p.N ? c0 + 8 : p.N - 1) * p.ldb;
+  const int steps = (int)((p.K + STEP - 1) / STEP);
+  uint4 wa[DEPTH], wb[DEPTH];
+  auto load_w = [&](int s0) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) {
+      const long long k = (long long)(s0 + d * KS) * STEP + 16 * t4;
+      wa[d] = load16(w0, k, p.K);
+      wb[d] = load16(w1, k, p.K);
+    }
+  };
+  load_w(ks);
+  tc::wait_predecessor();  // the tokens' codes and scales; the weight does not depend on them
+
+  const int pitch = (int)((p.K + 127) / 128 * 128) + 64;
+  int8_t* codes = reinterpret_cast<int8_t*>(dyn);
+  if (FUSED) {
+    const X* x = static_cast<const X*>(in.x);
+    __shared__ unsigned tops[SW];
+    for (int m = 0; m < (int)p.M; ++m)
+      quantize_row<X, 32 * SW>(codes + (long long)m * pitch, pitch - 64, &sa_s[m],
+                               x + m * in.ldx, (int)p.K, in.vec, tops);
+    __syncthreads();
+  }
+
+  for (long long m0 = lo; m0 < hi; m0 += TOKENS) {
+    const int have = hi - m0 < TOKENS ? (int)(hi - m0) : TOKENS;
+    if (!FUSED && threadIdx.x < TOKENS)
+      sa_s[threadIdx.x] = threadIdx.x < have ? p.sa[m0 + threadIdx.x] : 0.f;
+    int acc[MG][4];
+#pragma unroll
+    for (int j = 0; j < MG; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0;
+    for (int s0 = ks; s0 < steps; s0 += DEPTH * KS) {
+      if (s0 != ks || m0 != lo) load_w(s0);
+      uint4 tok[DEPTH][MG];
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        const long long k = (long long)(s0 + d * KS) * STEP + 16 * t4;
+#pragma unroll
+        for (int j = 0; j < MG; ++j) {
+          const int m = 8 * j + g;
+          tok[d][j] = make_uint4(0, 0, 0, 0);
+          if (m < have && k < p.K) {
+            if (FUSED) tok[d][j] = *reinterpret_cast<const uint4*>(codes + (long long)m * pitch + k);
+            else tok[d][j] = load16(p.a + (m0 + m) * p.lda, k, p.K);
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d)
+#pragma unroll
+        for (int j = 0; j < MG; ++j) {
+          mma_s8(acc[j], wa[d].x, wb[d].x, wa[d].y, wb[d].y, tok[d][j].x, tok[d][j].y);
+          mma_s8(acc[j], wa[d].z, wb[d].z, wa[d].w, wb[d].w, tok[d][j].z, tok[d][j].w);
+        }
+    }
+    // lane: channels g, g + 8; tokens 2 t4, 2 t4 + 1 of each group
+#pragma unroll
+    for (int j = 0; j < MG; ++j) {
+      red[ks][16 * rg + g][8 * j + 2 * t4] = acc[j][0];
+      red[ks][16 * rg + g][8 * j + 2 * t4 + 1] = acc[j][1];
+      red[ks][16 * rg + g + 8][8 * j + 2 * t4] = acc[j][2];
+      red[ks][16 * rg + g + 8][8 * j + 2 * t4 + 1] = acc[j][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < CHANNELS * have; i += 32 * SW) {
+      const int c = i % CHANNELS, m = i / CHANNELS;
+      const long long n = n0 + c;
+      if (n >= p.N) continue;
+      int sum = 0;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) sum += red[s][c][m];
+      out[(m0 + m) * p.ldo + n] = of_f<S>(
+          scaled(sum, sa_s[m], p.sb[group * p.N + n], p.bias ? p.bias[n] : 0.f));
+    }
+    if (m0 + TOKENS < hi) __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+
+// At most this many bytes of codes in a CTA's shared memory
+constexpr long long kFusedBytes = 40 * 1024;
+
+static long long fused_bytes(const Product& p) { return p.M * ((p.K + 127) / 128 * 128 + 64); }
+
+bool stream_takes(const Product& p) {
+  if (!tc_takes(p)) return false;  // the same alignment
+  // one group: two groups of eight tokens; groups: few rows each on average, so
+  // that hardly any weight is read more than once
+  return p.offsets ? p.M <= 2 * p.groups && p.M <= 4096 : p.M <= 16;
+}
+
+bool stream_quantizes(const Product& p) {
+  return stream_takes(p) && !p.offsets && p.M <= 4 && fused_bytes(p) <= kFusedBytes;
+}
+
+template <typename S, typename X, int RG, int MG, bool FUSED>
+static int launch_stream(const Product& p, const Input& in, bool overlap, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cdiv(p.N, 16 * RG), p.offsets ? (unsigned)(p.groups + 1) : 1, 1);
+  cfg.blockDim = dim3(32 * SW, 1, 1);
+  cfg.dynamicSmemBytes = FUSED ? (size_t)fused_bytes(p) : 0;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = overlap ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, stream_kernel<S, X, RG, MG, FUSED>, p, in);
+  g2q::note_launch();
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return G2Q_ERR_CUDA;
+  }
+  return G2Q_OK;
+}
+
+template <typename S>
+static int stream_out(const Product& p, bool overlap, cudaStream_t st) {
+  const Input none = {nullptr, 0, false};
+  if (p.offsets) return launch_stream<S, float, 4, 1, false>(p, none, overlap, st);
+  if (p.M <= 8) return launch_stream<S, float, 1, 1, false>(p, none, overlap, st);
+  return launch_stream<S, float, 1, 2, false>(p, none, overlap, st);
+}
+
+int stream_product(const Product& p, bool overlap, cudaStream_t st) {
+  if (p.out_dtype == G2Q_DTYPE_BF16) return stream_out<__nv_bfloat16>(p, overlap, st);
+  if (p.out_dtype == G2Q_DTYPE_F16) return stream_out<__half>(p, overlap, st);
+  return stream_out<float>(p, overlap, st);
+}
+
+template <typename X>
+static int stream_in(const Product& p, const Input& in, cudaStream_t st) {
+  if (p.out_dtype == G2Q_DTYPE_BF16)
+    return launch_stream<__nv_bfloat16, X, 1, 1, true>(p, in, false, st);
+  if (p.out_dtype == G2Q_DTYPE_F16) return launch_stream<__half, X, 1, 1, true>(p, in, false, st);
+  return launch_stream<float, X, 1, 1, true>(p, in, false, st);
+}
+
+int stream_linear(const Product& p, const void* x, int x_dtype, long long ldx, cudaStream_t st) {
+  const Input in = {x, ldx,
+                    rows::aligned(x, 16) &&
+                        (p.M <= 1 || ldx * rows::elem_bytes(x_dtype) % 16 == 0)};
+  if (x_dtype == G2Q_DTYPE_BF16) return stream_in<__nv_bfloat16>(p, in, st);
+  if (x_dtype == G2Q_DTYPE_F16) return stream_in<__half>(p, in, st);
+  return stream_in<float>(p, in, st);
+}
+
+}  // namespace i8
+}  // namespace g2q
