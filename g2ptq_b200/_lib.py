@@ -98,7 +98,7 @@ SIGNATURES = {
                                 P],
     "g2q_int8_linear": [P, I32, I64, P, I32, I64, P, I64, I64, P, P, P, I64, I64, I64, I64, P, SZ,
                         P, P],
-    "g2q_int8_linear_workspace_bytes": [I64, I64, I64, I64],
+    "g2q_int8_linear_workspace_bytes": [I64, I64, I64, I64, I32],
     "g2q_route": [P, P, P, P, I32, I64, I64, P, SZ, P],
     "g2q_route_workspace_bytes": [I64, I64],
     "g2q_dispatch_rows": [P, I64, P, I64, I32, P, I64, I64, I64, P],

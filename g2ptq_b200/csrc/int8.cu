@@ -220,8 +220,10 @@ static size_t product_workspace(const Product& p) {
 
 static size_t up256(size_t v) { return (v + 255) / 256 * 256; }
 
-// Workspace of a linear: the tokens' codes, their scales, the product's own.
+// Workspace of a linear whose weight is aligned: the tokens' codes, their scales,
+// the product's own.
 static size_t linear_workspace(const Product& p) {
+  if (stream_quantizes(p)) return 0;
   const size_t M = (size_t)p.M, ld = (size_t)((p.K + 15) / 16 * 16);
   return up256(M * ld) + up256(M * sizeof(float)) + product_workspace(p);
 }
@@ -289,11 +291,13 @@ extern "C" int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, co
   return i8::product(p, nullptr, 0, false, (cudaStream_t)stream);
 }
 
-extern "C" size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G) {
+extern "C" size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G,
+                                                  int aligned) {
   if (M <= 0 || N <= 0 || K <= 0 || G < 0 || K > i8::kMaxK || M > i8::kMaxRows ||
       N > i8::kMaxRows || G > i8::kMaxGroups)
     return 0;
   i8::Product p = {};
+  p.b = reinterpret_cast<const int8_t*>(aligned ? 256 : 257);
   p.lda = p.ldb = (K + 15) / 16 * 16;
   p.b_gs = p.ldb * N;
   p.groups = G > 0 ? G : 1;
@@ -313,13 +317,14 @@ extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void
   if (!rows::elem_bytes(x_dtype) || ldx < K || G < 0 || (G > 0) != (offsets != nullptr) ||
       (G > 0 && bias))
     return G2Q_ERR_INVALID_ARG;
-  // the operands that the workspace will hold stand in for the check
-  i8::Product p = {out, out_dtype, ldo, static_cast<int8_t*>(workspace), ld,
-                   static_cast<float*>(workspace), b, ldb, b_gs, b_scale, bias, offsets,
+  // aligned stand-ins for the operands that the workspace will hold
+  i8::Product p = {out, out_dtype, ldo, reinterpret_cast<int8_t*>(256), ld,
+                   reinterpret_cast<float*>(256), b, ldb, b_gs, b_scale, bias, offsets,
                    G > 0 ? G : 1, M, N, K, status};
   G2Q_TRY(i8::check(p));
   if (M == 0) return G2Q_OK;
-  if (!x || !rows::aligned(workspace, 16) || workspace_bytes < i8::linear_workspace(p))
+  const size_t need = i8::linear_workspace(p);
+  if (!x || (need && (!workspace || !rows::aligned(workspace, 16) || workspace_bytes < need)))
     return G2Q_ERR_INVALID_ARG;
   if (i8::stream_quantizes(p))
     return i8::stream_linear(p, x, x_dtype, ldx, (cudaStream_t)stream);
@@ -327,6 +332,7 @@ extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void
   const size_t code_bytes = i8::up256((size_t)M * (size_t)ld);
   const size_t scale_bytes = i8::up256((size_t)M * sizeof(float));
   float* scale = reinterpret_cast<float*>(ws + code_bytes);
+  p.a = reinterpret_cast<int8_t*>(ws);
   p.sa = scale;
   G2Q_TRY(i8::quantize_tokens(reinterpret_cast<int8_t*>(ws), ld, scale, x, x_dtype, ldx, M, K,
                               (cudaStream_t)stream));

@@ -4,14 +4,14 @@
 // microseconds on TMEM, clusters, the ring and a second kernel for K ranges.
 //
 // A CTA of eight warps takes 16 * RG channels; the warps of one 16-channel group
-// share K in turns of 64 bytes.  A lane loads 16 bytes of channels g and g + 8
+// share K in turns of 64 * DEPTH bytes.  A lane loads 16 bytes of channels g and g + 8
 // (g = lane / 4) and 16 bytes of token g, and multiplies them with two
 // mma.sync.m16n8k32 (int8): the order of K inside a step is free as long as both
 // operands use the same, so 16 consecutive bytes serve as the four words that a
 // lane owes two steps.  The warps' integer sums meet in shared memory.
 //
-// With few enough tokens the kernel quantizes them itself (FUSED): every CTA
-// makes the codes of all tokens in shared memory, behind its first weight loads.
+// A single token's codes are made by the kernel itself (FUSED): every CTA makes
+// them in shared memory, behind its first weight loads.
 #include "int8.cuh"
 #include "int8_quant.cuh"
 #include "tc_ptx.cuh"
@@ -46,6 +46,38 @@ __device__ __forceinline__ uint4 load16(const int8_t* row, long long k, long lon
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// The slot-th group that has rows (counting the rows behind the last group as
+// one more); false where there are fewer.  By each warp alone.
+__device__ __forceinline__ bool find_group(const Product& p, int slot, int* group, long long* lo,
+                                           long long* hi) {
+  const int lane = threadIdx.x & 31;
+  for (int g0 = 0; g0 <= p.groups; g0 += 128) {
+    long long from[4], to[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      from[i] = to[i] = 0;
+      if (g0 + 32 * i + lane <= p.groups)
+        group_bounds(p, g0 + 32 * i + lane, &from[i], &to[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned has = __ballot_sync(0xffffffffu, to[i] > from[i]);
+      const int count = __popc(has);
+      if (slot < count) {
+        // the lane with `slot` set lanes before it
+        const bool mine = (has >> lane & 1u) && __popc(has & ((1u << lane) - 1u)) == slot;
+        const int src = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;
+        *group = g0 + 32 * i + src;
+        *lo = __shfl_sync(0xffffffffu, from[i], src);
+        *hi = __shfl_sync(0xffffffffu, to[i], src);
+        return true;
+      }
+      slot -= count;
+    }
+  }
+  return false;
+}
+
 struct Input {  // the tokens before quantization (FUSED)
   const void* x;
   long long ldx;
@@ -61,14 +93,13 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
   __shared__ float sa_s[TOKENS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rg = warp % RG, ks = warp / RG, g = lane / 4, t4 = lane % 4;
-  const long long group = p.offsets ? blockIdx.y : 0;
+  int group = 0;
   const long long n0 = (long long)blockIdx.x * CHANNELS;
   long long lo = 0, hi = p.M;
   if (p.offsets) {
-    group_bounds(p, group, &lo, &hi);
     // the grid ends after the kernel before it even if no CTA has rows
     if (blockIdx.x == 0 && blockIdx.y == 0) tc::wait_predecessor();
-    if (lo == hi) return;
+    if (!find_group(p, blockIdx.y, &group, &lo, &hi)) return;
   }
   S* out = static_cast<S*>(p.out);
   if (group == p.groups) {  // rows behind the last group
@@ -78,17 +109,18 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
     }
     return;
   }
-  const int8_t* b = p.b + group * p.b_gs;
+  const int8_t* b = p.b + (long long)group * p.b_gs;
   const long long c0 = n0 + 16 * rg + g;
   // channels that do not exist read the last one's bytes; their sums go nowhere
   const int8_t* w0 = b + (c0 < p.N ? c0 : p.N - 1) * p.ldb;
   const int8_t* w1 = b + (c0 + 8 < p.N ? c0 + 8 : p.N - 1) * p.ldb;
-  const int steps = (int)((p.K + STEP - 1) / STEP);
+  // a warp's steps in flight are neighbours in K: 64 * DEPTH bytes of each row
+  const int turns = (int)((p.K + STEP * DEPTH - 1) / (STEP * DEPTH));
   uint4 wa[DEPTH], wb[DEPTH];
-  auto load_w = [&](int s0) {
+  auto load_w = [&](int turn) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      const long long k = (long long)(s0 + d * KS) * STEP + 16 * t4;
+      const long long k = ((long long)turn * DEPTH + d) * STEP + 16 * t4;
       wa[d] = load16(w0, k, p.K);
       wb[d] = load16(w1, k, p.K);
     }
@@ -116,12 +148,12 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
     for (int j = 0; j < MG; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[j][i] = 0;
-    for (int s0 = ks; s0 < steps; s0 += DEPTH * KS) {
-      if (s0 != ks || m0 != lo) load_w(s0);
+    for (int turn = ks; turn < turns; turn += KS) {
+      if (turn != ks || m0 != lo) load_w(turn);
       uint4 tok[DEPTH][MG];
 #pragma unroll
       for (int d = 0; d < DEPTH; ++d) {
-        const long long k = (long long)(s0 + d * KS) * STEP + 16 * t4;
+        const long long k = ((long long)turn * DEPTH + d) * STEP + 16 * t4;
 #pragma unroll
         for (int j = 0; j < MG; ++j) {
           const int m = 8 * j + g;
@@ -157,7 +189,7 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
 #pragma unroll
       for (int s = 0; s < KS; ++s) sum += red[s][c][m];
       out[(m0 + m) * p.ldo + n] = of_f<S>(
-          scaled(sum, sa_s[m], p.sb[group * p.N + n], p.bias ? p.bias[n] : 0.f));
+          scaled(sum, sa_s[m], p.sb[(long long)group * p.N + n], p.bias ? p.bias[n] : 0.f));
     }
     if (m0 + TOKENS < hi) __syncthreads();
   }
@@ -167,8 +199,10 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
 // host side
 // ---------------------------------------------------------------------------
 
-// At most this many bytes of codes in a CTA's shared memory
-constexpr long long kFusedBytes = 40 * 1024;
+// Longest row that every CTA quantizes for itself: 4096 columns took 5.0 us with
+// and 5.3 us without the separate kernel, 14336 columns 16.9 and 15.5 us; four
+// tokens of 4096 columns 8.2 and 5.3 us.
+constexpr long long kFusedColumns = 8192;
 
 static long long fused_bytes(const Product& p) { return p.M * ((p.K + 127) / 128 * 128 + 64); }
 
@@ -176,17 +210,21 @@ bool stream_takes(const Product& p) {
   if (!tc_takes(p)) return false;  // the same alignment
   // one group: two groups of eight tokens; groups: few rows each on average, so
   // that hardly any weight is read more than once
-  return p.offsets ? p.M <= 2 * p.groups && p.M <= 4096 : p.M <= 16;
+  if (p.offsets) return p.M <= 2 * p.groups && p.M <= 4096;
+  // more than eight tokens double the work per weight byte: 14336 channels x 4096
+  // took 20.6 us here and 17.1 us on the tiles, 4096 x 4096 6.4 and 11.5 us
+  return p.M <= (p.N <= 8192 ? 16 : 8);
 }
 
 bool stream_quantizes(const Product& p) {
-  return stream_takes(p) && !p.offsets && p.M <= 4 && fused_bytes(p) <= kFusedBytes;
+  return stream_takes(p) && !p.offsets && p.M == 1 && p.K <= kFusedColumns;
 }
 
 template <typename S, typename X, int RG, int MG, bool FUSED>
 static int launch_stream(const Product& p, const Input& in, bool overlap, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cdiv(p.N, 16 * RG), p.offsets ? (unsigned)(p.groups + 1) : 1, 1);
+  cfg.gridDim = dim3((unsigned)cdiv(p.N, 16 * RG), 
+                     p.offsets ? (unsigned)(p.groups < p.M ? p.groups + 1 : p.M) : 1, 1);
   cfg.blockDim = dim3(32 * SW, 1, 1);
   cfg.dynamicSmemBytes = FUSED ? (size_t)fused_bytes(p) : 0;
   cfg.stream = st;

@@ -545,40 +545,57 @@ INT8_MAX_K = 131071  # |a b| <= 128 * 128: longer sums could leave 32 bits
 MAX_EXPERTS = 1024
 
 
-def _call_on(device, name, *args):
-    """``call`` with ``device`` current: a kernel is launched on the current
-    device, which need not be the tensors'."""
-    if torch.cuda.current_device() == device.index:
-        return call(name, *args)
-    with torch.cuda.device(device):
-        return call(name, *args)
+def _device_of(*tensors):
+    """Index of the CUDA device that every given tensor (None: skipped) is on;
+    ``_cuda``'s errors."""
+    idx = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and (idx < 0 or t.get_device() != idx):
+            _cuda(*tensors)
+    return idx
 
 
-def _raw_stream(device):
-    """The current stream of ``device`` as ``_stream`` gives it, without the
-    Stream object (a tenth of a microsecond instead of two)."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _call_on(idx, name, *args):
+    """``call`` with device ``idx`` current and its current stream as the last
+    argument: a kernel is launched on the current device, which need not be the
+    tensors'."""
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if torch.cuda.current_device() == idx:
+        return call(name, *args, stream)
+    with torch.cuda.device(idx):
+        return call(name, *args, stream)
+
+
+def _status_word(idx):
+    t = _DEVICE_STATUS.get(idx)
+    return (device_status(torch.device("cuda", idx)) if t is None else t).data_ptr()
+
+
+def _rows_bytes(nbytes, like):
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _matrix(name, t):
-    """Row stride of the 2-D ``t`` with unit column stride and rows that do not overlap."""
+    """``(rows, columns, row stride)`` of the 2-D ``t`` with unit column stride and
+    rows that do not overlap."""
     if t.dim() != 2:
         raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
     rows, cols = t.shape
-    if cols > 1 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
         raise ValueError(f"{name} needs unit column stride")
     if rows <= 1:
-        return max(cols, 1)
-    if t.stride(0) < cols:
+        return rows, cols, max(cols, 1)
+    if ld < cols:
         raise ValueError(f"{name} has overlapping rows")
-    return t.stride(0)
+    return rows, cols, ld
 
 
 def _vector(name, t, n, dtype=torch.float32):
-    if t.shape != (n,) or t.dtype != dtype:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
         raise ValueError(f"{name} must be {dtype} of shape ({n},), got {t.dtype} of shape "
                          f"{tuple(t.shape)}")
-    if not t.is_contiguous():
+    if n > 1 and t.stride(0) != 1:
         raise ValueError(f"{name} must be contiguous")
 
 
@@ -594,62 +611,79 @@ def quantize_tokens(x):
     even.  A row whose values are all zero has scale 1; one with an infinity or
     a NaN has scale NaN and codes 0.  Returns ``(codes [T, C], scale [T])``, the
     codes' rows ``int8_row_stride(C)`` apart."""
-    dev = _cuda(x)
-    ldx = _matrix("x", x)
-    T, C = x.shape
+    idx = _device_of(x)
+    T, C, ldx = _matrix("x", x)
     if C == 0:
         raise ValueError("quantize_tokens needs at least one column")
+    dt = dtype_code(x.dtype)
     ldq = int8_row_stride(C)
-    codes = torch.empty(T, ldq, dtype=torch.int8, device=dev)[:, :C]
-    scale = torch.empty(T, dtype=torch.float32, device=dev)
-    _call_on(dev, "g2q_quantize_tokens", codes.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(),
-             dtype_code(x.dtype), ldx, T, C, _raw_stream(dev))
+    codes = x.new_empty((T, ldq), dtype=torch.int8)[:, :C]
+    scale = x.new_empty(T, dtype=torch.float32)
+    _call_on(idx, "g2q_quantize_tokens", codes.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(), dt,
+             ldx, T, C)
     return codes, scale
+
+
+def _weight(b, b_scale, K):
+    """``(N, ldb)`` of int8 codes ``b [N, K]`` with their scales."""
+    if b.dtype != torch.int8:
+        raise TypeError(f"the weight must be int8 codes, got {b.dtype}")
+    N, Kb, ldb = _matrix("b", b)
+    if Kb != K:
+        raise ValueError(f"the tokens have {K} columns and the weight {Kb}")
+    if not 0 < K <= INT8_MAX_K or N == 0:
+        raise ValueError(f"needs 1 to {INT8_MAX_K} columns and at least one channel")
+    _vector("b_scale", b_scale, N)
+    return N, ldb
+
+
+def _expert_weight(b, b_scale, offsets, K):
+    """``(E, N, ldb, b_gs)`` of the stacked codes ``b [E, N, K]``."""
+    if b.dtype != torch.int8:
+        raise TypeError(f"the weight must be int8 codes, got {b.dtype}")
+    if b.dim() != 3:
+        raise ValueError(f"b must be [experts, channels, columns], got shape {tuple(b.shape)}")
+    E, N, Kb = b.shape
+    if Kb != K:
+        raise ValueError(f"the rows have {K} columns and the weight {Kb}")
+    if not 0 < K <= INT8_MAX_K or N == 0 or not 0 < E <= MAX_EXPERTS:
+        raise ValueError(f"needs 1 to {INT8_MAX_K} columns, at least one channel and 1 to "
+                         f"{MAX_EXPERTS} experts")
+    gs, ld, step = b.stride()
+    ldb = ld if N > 1 else K
+    if (K > 1 and step != 1) or ldb < K or (E > 1 and gs < N * ldb):
+        raise ValueError("b needs unit column stride and experts and rows that do not overlap")
+    if b_scale.dtype != torch.float32 or b_scale.shape != (E, N) or not b_scale.is_contiguous():
+        raise ValueError(f"b_scale must be contiguous fp32 of shape ({E}, {N})")
+    _vector("offsets", offsets, E + 1, torch.int32)
+    return E, N, ldb, gs if E > 1 else N * ldb
+
+
+def _codes(a, a_scale):
+    if a.dtype != torch.int8:
+        raise TypeError(f"the tokens must be int8 codes, got {a.dtype}")
+    M, K, lda = _matrix("a", a)
+    _vector("a_scale", a_scale, M)
+    return M, K, lda
 
 
 def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
     """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k] + bias[n]``
     for int8 ``a [M, K]`` and ``b [N, K]``, fp32 scales and bias; the sums are
     exact.  Rows 16 bytes aligned (``int8_row_stride``) run on the tensor cores."""
-    dev = _cuda(a, a_scale, b, b_scale, bias)
-    lda, ldb = _matrix("a", a), _matrix("b", b)
-    if a.dtype != torch.int8 or b.dtype != torch.int8:
-        raise TypeError("int8_matmul takes int8 codes")
-    M, K = a.shape
-    N = b.shape[0]
-    if b.shape[1] != K:
-        raise ValueError(f"a has {K} columns and b {b.shape[1]}")
-    if not 0 < K <= INT8_MAX_K or N == 0:
-        raise ValueError(f"int8_matmul needs 1 to {INT8_MAX_K} columns and at least one channel")
-    _vector("a_scale", a_scale, M)
-    _vector("b_scale", b_scale, N)
+    idx = _device_of(a, a_scale, b, b_scale, bias)
+    M, K, lda = _codes(a, a_scale)
+    N, ldb = _weight(b, b_scale, K)
     if bias is not None:
         _vector("bias", bias, N)
-    out = torch.empty(M, N, dtype=out_dtype, device=dev)
+    dt = dtype_code(out_dtype)
+    out = a.new_empty((M, N), dtype=out_dtype)
     ws_bytes = query("g2q_int8_matmul_workspace_bytes", M, N, K)
-    ws = workspace(ws_bytes, dev) if ws_bytes else None
-    _call_on(dev, "g2q_int8_matmul", out.data_ptr(), dtype_code(out_dtype), N, a.data_ptr(), lda,
-             a_scale.data_ptr(), b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K,
-             _ptr(ws), ws_bytes, _status(None, dev), _raw_stream(dev))
+    ws = _rows_bytes(ws_bytes, a)
+    _call_on(idx, "g2q_int8_matmul", out.data_ptr(), dt, N, a.data_ptr(), lda, a_scale.data_ptr(),
+             b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K, _ptr(ws), ws_bytes,
+             _status_word(idx))
     return out
-
-
-def _expert_weight(b, b_scale, K):
-    """``(N, ldb, b_gs)`` of the stacked codes ``b [E, N, K]``."""
-    if b.dim() != 3:
-        raise ValueError(f"b must be [experts, channels, columns], got shape {tuple(b.shape)}")
-    E, N, Kb = b.shape
-    if Kb != K:
-        raise ValueError(f"a has {K} columns and b {Kb}")
-    if not 0 < K <= INT8_MAX_K or N == 0 or not 0 < E <= MAX_EXPERTS:
-        raise ValueError(f"needs 1 to {INT8_MAX_K} columns, at least one channel and 1 to "
-                         f"{MAX_EXPERTS} experts")
-    ldb = b.stride(1) if N > 1 else K
-    if (K > 1 and b.stride(2) != 1) or ldb < K or (E > 1 and b.stride(0) < N * ldb):
-        raise ValueError("b needs unit column stride and experts and rows that do not overlap")
-    if b_scale.shape != (E, N) or b_scale.dtype != torch.float32 or not b_scale.is_contiguous():
-        raise ValueError(f"b_scale must be contiguous fp32 of shape ({E}, {N})")
-    return N, ldb, b.stride(0) if E > 1 else N * ldb
 
 
 def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat16):
@@ -657,65 +691,49 @@ def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat1
     ``offsets[e + 1] - 1`` of ``a [R, K]`` are multiplied with ``b[e]`` of
     ``b [E, N, K]`` and scaled by ``b_scale [E, N]``.  ``offsets`` is int32
     ``[E + 1]``, ascending from 0; rows behind ``offsets[E]`` give zeros."""
-    dev = _cuda(a, a_scale, b, b_scale, offsets)
-    lda = _matrix("a", a)
-    if a.dtype != torch.int8 or b.dtype != torch.int8:
-        raise TypeError("int8_matmul_grouped takes int8 codes")
-    R, K = a.shape
-    N, ldb, b_gs = _expert_weight(b, b_scale, K)
-    _vector("a_scale", a_scale, R)
-    _vector("offsets", offsets, b.shape[0] + 1, torch.int32)
-    out = torch.empty(R, N, dtype=out_dtype, device=dev)
-    _call_on(dev, "g2q_int8_matmul_grouped", out.data_ptr(), dtype_code(out_dtype), N,
-             a.data_ptr(), lda, a_scale.data_ptr(), b.data_ptr(), ldb, b_gs, b_scale.data_ptr(),
-             offsets.data_ptr(), b.shape[0], R, N, K, _status(None, dev), _raw_stream(dev))
+    idx = _device_of(a, a_scale, b, b_scale, offsets)
+    R, K, lda = _codes(a, a_scale)
+    E, N, ldb, b_gs = _expert_weight(b, b_scale, offsets, K)
+    dt = dtype_code(out_dtype)
+    out = a.new_empty((R, N), dtype=out_dtype)
+    _call_on(idx, "g2q_int8_matmul_grouped", out.data_ptr(), dt, N, a.data_ptr(), lda,
+             a_scale.data_ptr(), b.data_ptr(), ldb, b_gs, b_scale.data_ptr(), offsets.data_ptr(),
+             E, R, N, K, _status_word(idx))
     return out
 
 
 def int8_linear(x, codes, scale, bias=None):
     """``quantize_tokens`` of ``x [M, K]`` and ``int8_matmul`` with ``codes [N, K]``
     in one call; the result has ``x``'s type."""
-    dev = _cuda(x, codes, scale, bias)
-    ldx, ldb = _matrix("x", x), _matrix("codes", codes)
-    if codes.dtype != torch.int8:
-        raise TypeError("int8_linear takes int8 codes")
-    M, K = x.shape
-    N, Kb = codes.shape
-    if Kb != K:
-        raise ValueError(f"x has {K} columns and codes {Kb}")
-    if not 0 < K <= INT8_MAX_K or N == 0:
-        raise ValueError(f"int8_linear needs 1 to {INT8_MAX_K} columns and at least one channel")
-    _vector("scale", scale, N)
+    idx = _device_of(x, codes, scale, bias)
+    M, K, ldx = _matrix("x", x)
+    N, ldb = _weight(codes, scale, K)
     if bias is not None:
         _vector("bias", bias, N)
     dt = dtype_code(x.dtype)
-    out = torch.empty(M, N, dtype=x.dtype, device=dev)
-    ws_bytes = query("g2q_int8_linear_workspace_bytes", M, N, K, 0)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call_on(dev, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx,
-             codes.data_ptr(), ldb, 0, scale.data_ptr(), _ptr(bias), None, 0, M, N, K,
-             ws.data_ptr(), ws_bytes, _status(None, dev), _raw_stream(dev))
+    out = x.new_empty((M, N))
+    b = codes.data_ptr()
+    ws_bytes = query("g2q_int8_linear_workspace_bytes", M, N, K, 0, (b | ldb) % 16 == 0)
+    ws = _rows_bytes(ws_bytes, x)
+    _call_on(idx, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx, b, ldb, 0,
+             scale.data_ptr(), _ptr(bias), None, 0, M, N, K, _ptr(ws), ws_bytes, _status_word(idx))
     return out
 
 
 def int8_linear_grouped(x, codes, scale, offsets):
     """``quantize_tokens`` of ``x [R, K]`` and ``int8_matmul_grouped`` with ``codes
     [E, N, K]`` in one call; the result has ``x``'s type."""
-    dev = _cuda(x, codes, scale, offsets)
-    ldx = _matrix("x", x)
-    if codes.dtype != torch.int8:
-        raise TypeError("int8_linear_grouped takes int8 codes")
-    R, K = x.shape
-    N, ldb, b_gs = _expert_weight(codes, scale, K)
-    E = codes.shape[0]
-    _vector("offsets", offsets, E + 1, torch.int32)
+    idx = _device_of(x, codes, scale, offsets)
+    R, K, ldx = _matrix("x", x)
+    E, N, ldb, b_gs = _expert_weight(codes, scale, offsets, K)
     dt = dtype_code(x.dtype)
-    out = torch.empty(R, N, dtype=x.dtype, device=dev)
-    ws_bytes = query("g2q_int8_linear_workspace_bytes", R, N, K, E)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    _call_on(dev, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx,
-             codes.data_ptr(), ldb, b_gs, scale.data_ptr(), None, offsets.data_ptr(), E, R, N, K,
-             ws.data_ptr(), ws_bytes, _status(None, dev), _raw_stream(dev))
+    out = x.new_empty((R, N))
+    b = codes.data_ptr()
+    ws_bytes = query("g2q_int8_linear_workspace_bytes", R, N, K, E, (b | ldb | b_gs) % 16 == 0)
+    ws = _rows_bytes(ws_bytes, x)
+    _call_on(idx, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx, b, ldb, b_gs,
+             scale.data_ptr(), None, offsets.data_ptr(), E, R, N, K, _ptr(ws), ws_bytes,
+             _status_word(idx))
     return out
 
 
@@ -730,61 +748,60 @@ def route(experts, num_experts):
     ``t k + j`` in expert order, every pair's row there, and each expert's first
     row.  Pairs whose id is not in ``[0, num_experts)`` come last and have
     position ``-1 - row``."""
-    dev = _cuda(experts)
+    idx = _device_of(experts)
     if experts.dim() != 2 or experts.shape[1] == 0:
         raise ValueError(f"experts must be [tokens, slots], got shape {tuple(experts.shape)}")
-    if experts.dtype not in (torch.int32, torch.int64):
+    wide = experts.dtype == torch.int64
+    if not wide and experts.dtype != torch.int32:
         raise TypeError(f"experts must be int32 or int64, got {experts.dtype}")
     if not 0 < num_experts <= MAX_EXPERTS:
         raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
     _contig(experts)
     n = experts.numel()
-    order = torch.empty(n, dtype=torch.int32, device=dev)
-    position = torch.empty(experts.shape, dtype=torch.int32, device=dev)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
+    order = experts.new_empty(n, dtype=torch.int32)
+    position = experts.new_empty(experts.shape, dtype=torch.int32)
+    offsets = experts.new_empty(num_experts + 1, dtype=torch.int32)
     ws_bytes = query("g2q_route_workspace_bytes", n, num_experts)
-    ws = workspace(ws_bytes, dev) if ws_bytes else None
-    _call_on(dev, "g2q_route", order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
-             experts.data_ptr(), int(experts.dtype == torch.int64), n, int(num_experts), _ptr(ws),
-             ws_bytes, _raw_stream(dev))
+    ws = _rows_bytes(ws_bytes, experts)
+    _call_on(idx, "g2q_route", order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
+             experts.data_ptr(), wide, n, num_experts, _ptr(ws), ws_bytes)
     return order, position, offsets
 
 
 def _positions(position):
-    if position.dim() != 2 or position.shape[1] == 0 or position.dtype != torch.int32:
+    if position.dtype != torch.int32 or position.dim() != 2 or position.shape[1] == 0:
         raise ValueError("position must be int32 [tokens, slots]")
-    _contig(position)
+    if not position.is_contiguous():
+        raise ValueError("position must be contiguous")
     return position.shape
+
+
+def _weights(weights, position):
+    """dtype code of the routing weights (0 for None)."""
+    if weights is None:
+        return 0
+    if weights.shape != position.shape:
+        raise ValueError(f"weights must have shape {tuple(position.shape)}")
+    if not weights.is_contiguous():
+        raise ValueError("weights must be contiguous")
+    return dtype_code(weights.dtype)
 
 
 def dispatch_rows(x, position):
     """Rows of ``x [T, C]`` (1-, 2- or 4-byte elements) copied to the rows that
     ``position [T, k]`` (of ``route``) gives each slot: ``[T k, C]``.  Rows of
     pairs without an expert are zero."""
-    dev = _cuda(x, position)
-    ldx = _matrix("x", x)
+    idx = _device_of(x, position)
     T, k = _positions(position)
-    if x.shape[0] != T or x.shape[1] == 0:
+    rows, C, ldx = _matrix("x", x)
+    if rows != T or C == 0:
         raise ValueError(f"x must have {T} rows and at least one column")
     if x.element_size() not in (1, 2, 4):
         raise TypeError(f"unsupported dtype {x.dtype}")
-    out = torch.empty(T * k, x.shape[1], dtype=x.dtype, device=dev)
-    _call_on(dev, "g2q_dispatch_rows", out.data_ptr(), x.shape[1], x.data_ptr(), ldx,
-             x.element_size(), position.data_ptr(), T, k, x.shape[1], _raw_stream(dev))
+    out = x.new_empty((T * k, C))
+    _call_on(idx, "g2q_dispatch_rows", out.data_ptr(), C, x.data_ptr(), ldx, x.element_size(),
+             position.data_ptr(), T, k, C)
     return out
-
-
-def _expert_rows(y, position, weights):
-    T, k = _positions(position)
-    ldy = _matrix("y", y)
-    if y.shape[0] != T * k or y.shape[1] == 0:
-        raise ValueError(f"y must have {T * k} rows and at least one column")
-    if weights is not None:
-        if weights.shape != position.shape:
-            raise ValueError(f"weights must have shape {tuple(position.shape)}")
-        dtype_code(weights.dtype)
-        _contig(weights)
-    return T, k, ldy
 
 
 def combine_rows(y, position, weights=None):
@@ -792,13 +809,15 @@ def combine_rows(y, position, weights=None):
     expert, added in slot order in fp32 and rounded once to ``y``'s type:
     ``y [T k, C]``, ``position [T, k]`` of ``route``, ``weights [T, k]`` (None:
     ones).  A token without any expert gives zeros."""
-    dev = _cuda(y, position, weights)
-    T, k, ldy = _expert_rows(y, position, weights)
-    C = y.shape[1]
-    out = torch.empty(T, C, dtype=y.dtype, device=dev)
-    _call_on(dev, "g2q_combine_rows", out.data_ptr(), C, y.data_ptr(), ldy, dtype_code(y.dtype),
-             position.data_ptr(), _ptr(weights), 0 if weights is None else dtype_code(weights.dtype),
-             T, k, C, _raw_stream(dev))
+    idx = _device_of(y, position, weights)
+    T, k = _positions(position)
+    rows, C, ldy = _matrix("y", y)
+    if rows != T * k or C == 0:
+        raise ValueError(f"y must have {T * k} rows and at least one column")
+    dt, wdt = dtype_code(y.dtype), _weights(weights, position)
+    out = y.new_empty((T, C))
+    _call_on(idx, "g2q_combine_rows", out.data_ptr(), C, y.data_ptr(), ldy, dt,
+             position.data_ptr(), _ptr(weights), wdt, T, k, C)
     return out
 
 
@@ -808,23 +827,21 @@ def combine_rows_backward(grad, y, position, weights, need_y=True, need_weights=
     read for the weights' gradient alone).  Rows and weights of pairs without an
     expert get zero."""
     y = y if need_weights else None
-    dev = _cuda(grad, y, position, weights)
+    idx = _device_of(grad, y, position, weights)
     T, k = _positions(position)
-    ldg = _matrix("grad", grad)
-    C = grad.shape[1]
-    if grad.shape[0] != T or C == 0:
+    rows, C, ldg = _matrix("grad", grad)
+    if rows != T or C == 0:
         raise ValueError(f"grad must have {T} rows and at least one column")
-    if weights is None or weights.shape != position.shape:
-        raise ValueError(f"weights must have shape {tuple(position.shape)}")
-    _contig(weights)
+    if weights is None:
+        raise ValueError("combine_rows_backward needs the weights")
+    dt, wdt = dtype_code(grad.dtype), _weights(weights, position)
     ldy = C
     if y is not None:
-        ldy = _matrix("y", y)
-        if y.shape != (T * k, C) or y.dtype != grad.dtype:
+        yr, yc, ldy = _matrix("y", y)
+        if yr != T * k or yc != C or y.dtype != grad.dtype:
             raise ValueError(f"y must be {grad.dtype} of shape ({T * k}, {C})")
-    gy = torch.empty(T * k, C, dtype=grad.dtype, device=dev) if need_y else None
-    gw = torch.empty(T, k, dtype=weights.dtype, device=dev) if need_weights else None
-    _call_on(dev, "g2q_combine_rows_backward", _ptr(gy), C, _ptr(gw), grad.data_ptr(), ldg,
-             _ptr(y), ldy, dtype_code(grad.dtype), position.data_ptr(), weights.data_ptr(),
-             dtype_code(weights.dtype), T, k, C, _raw_stream(dev))
+    gy = grad.new_empty((T * k, C)) if need_y else None
+    gw = torch.empty_like(weights) if need_weights else None
+    _call_on(idx, "g2q_combine_rows_backward", _ptr(gy), C, _ptr(gw), grad.data_ptr(), ldg,
+             _ptr(y), ldy, dt, position.data_ptr(), weights.data_ptr(), wdt, T, k, C)
     return gy, gw

@@ -489,9 +489,10 @@ int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t*
 
 /* g2q_quantize_tokens of x [M, K] (type x_dtype) followed by g2q_int8_matmul
  * (G = 0, offsets NULL) or g2q_int8_matmul_grouped (G > 0, bias NULL) in one
- * call, the product starting while the quantization ends.  `workspace`: g2q_int8_linear_workspace_bytes(M, N, K, G) bytes, 16-byte
- * aligned. */
-size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G);
+ * call, the product starting while the quantization ends.  `workspace`: 16-byte
+ * aligned, g2q_int8_linear_workspace_bytes(M, N, K, G, aligned) bytes (may be 0),
+ * with aligned != 0 only where b's base and strides are multiples of 16 bytes. */
+size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G, int aligned);
 int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void* x, int x_dtype, int64_t ldx,
                     const int8_t* b, int64_t ldb, int64_t b_gs, const float* b_scale,
                     const float* bias, const int32_t* offsets, int64_t G, int64_t M, int64_t N,
