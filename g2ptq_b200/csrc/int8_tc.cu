@@ -42,14 +42,26 @@ constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int STRIP_BYTES = 16 * 32 * 2;  // 16 tokens x 32 channels of 2 bytes
 constexpr int RASTER = 8;            // row pieces walked together (4 and 16 measured the same)
-constexpr int BAR_BYTES = 128;       // barriers, TMEM address, abort flag
+constexpr int BAR_BYTES = 256;       // barriers, TMEM address, abort flag
 static_assert((2 * STAGES + 5) * 8 + 8 <= BAR_BYTES, "barrier area");
+
+// Tensor maps: the weight as [group][chunk][channel][128 bytes] and the tokens as
+// [chunk][row][128 bytes] in boxes of KC chunks, the tokens' 32, 64, 96 and 128
+// rows high (what a CTA's half of a piece can need; a box is one load and lies
+// in shared memory as the MMAs read it).  Where K ends inside a chunk the chunk
+// dimension would run into the next row: then K is the innermost dimension and
+// the boxes are single chunks.
+struct Maps {
+  CUtensorMap w, t[4];
+};
 
 struct TcArgs {
   Product p;
   int tok;                       // tokens per tile: 64, 128 or 256
   int ch_tiles, nk;              // channel tiles; chunks of K
   int splits, per_split;         // K ranges and chunks in each
+  int wide;                      // K is whole chunks: one load per operand and stage
+  float per_band;                // 1 / (RASTER * ch_tiles)
   int32_t* part;                 // [splits][M][N] when splits > 1
   long long wait_cycles;
 };
@@ -91,7 +103,11 @@ __device__ __forceinline__ void build_table(const Product& p, int tok, const Tab
   }
 }
 
+// By a whole warp (every lane gets the tile): the way to the next tile is on the
+// producer's and the MMA issuer's critical path, so the group is found with two
+// ballots and the divisions are few.
 __device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, int w) {
+  const int lane = threadIdx.x & 31;
   Tile r;
   r.split = 0;
   if (a.splits > 1) {
@@ -99,20 +115,37 @@ __device__ __forceinline__ Tile decode(const TcArgs& a, const Table& t, int w) {
     w /= a.splits;
   }
   const int groups = (int)a.p.groups, pieces = t.first[groups + 1];
-  const int r0 = w / (RASTER * a.ch_tiles) * RASTER;
-  const int gsz = pieces - r0 < RASTER ? pieces - r0 : RASTER;
-  const int rem = w - r0 * a.ch_tiles;
-  const int piece = r0 + rem % gsz;
-  r.ch0 = rem / gsz * CH;
-  int lo = 0, hi = groups;  // the last group with first <= piece
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (t.first[mid] <= piece) lo = mid;
-    else hi = mid - 1;
+  const int band = RASTER * a.ch_tiles;
+  int b = (int)((float)w * a.per_band);  // w / band, off by one at most
+  b -= b * band > w;
+  b += (b + 1) * band <= w;
+  const int r0 = b * RASTER, rem = w - b * band;
+  const int gsz = pieces - r0;
+  int ch, piece;
+  if (gsz >= RASTER) {
+    ch = rem / RASTER;
+    piece = r0 + rem % RASTER;
+  } else {
+    ch = rem / gsz;
+    piece = r0 + (rem - ch * gsz);
   }
-  r.group = lo;
-  r.row0 = t.lo[lo] + (piece - t.first[lo]) * a.tok;
-  const int left = t.lo[lo + 1] - r.row0;
+  r.ch0 = ch * CH;
+  // the last group with first <= piece: first among every 32nd, then in its stretch
+  int g = 0;
+  if (groups > 1) {
+    const unsigned coarse =
+        __ballot_sync(0xffffffffu, 32 * lane <= groups && t.first[32 * lane] <= piece);
+    g = 32 * (31 - __clz(coarse));
+    const unsigned fine =
+        __ballot_sync(0xffffffffu, g + lane <= groups && t.first[g + lane] <= piece);
+    g += 31 - __clz(fine);
+    if (groups == 1024 && t.first[1024] <= piece) g = 1024;
+  } else if (t.first[1] <= piece) {
+    g = 1;
+  }
+  r.group = g;
+  r.row0 = t.lo[g] + (piece - t.first[g]) * a.tok;
+  const int left = t.lo[g + 1] - r.row0;
   r.rows = left < a.tok ? left : a.tok;
   r.k0 = r.split * a.per_split;
   r.k1 = r.k0 + a.per_split < a.nk ? r.k0 + a.per_split : a.nk;
@@ -149,6 +182,14 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(mbar_cluster)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_4d_pair(uint32_t dst, const CUtensorMap* map, int x, int y,
+                                                 int z, int w, uint32_t mbar_cluster) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(mbar_cluster)
       : "memory");
 }
 
@@ -194,8 +235,7 @@ struct Channels {
 
 template <typename S>
 __global__ void __launch_bounds__(THREADS, 1)
-    tc_kernel(const __grid_constant__ CUtensorMap mw, const __grid_constant__ CUtensorMap mt128,
-              const __grid_constant__ CUtensorMap mt32, const TcArgs a) {
+    tc_kernel(const __grid_constant__ Maps maps, const TcArgs a) {
   const Product& p = a.p;
   const uint32_t rank = cluster_ctarank();
   extern __shared__ uint8_t smem_raw[];
@@ -252,58 +292,63 @@ __global__ void __launch_bounds__(THREADS, 1)
   launch_dependents();  // the finishing kernel, which waits for this one to end
   int issued = 0;  // stages whose loads this CTA's producer issued
   if (warp == 0) {
-    if (lane == 0) {
-      const uint32_t full_lead = mapa_shared(full0, 0);
-      // loads of chunks k .. of tile t into stage s: the weight's, the tokens'
-      auto load_w = [&](const Tile& t, int k, int s) {
-        const int nc = t.k1 - k < KC ? t.k1 - k : KC, half = mma_n(t.rows) / 2;
-        // the leader's full[s] expects the bytes of both CTAs
-        if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * nc * (OP_BYTES + half * KB));
-        const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+    const uint32_t full_lead = mapa_shared(full0, 0);
+    // loads of chunks k .. of tile t into stage s (lane 0): the weight's, the tokens'
+    auto load_w = [&](const Tile& t, int k, int s) {
+      const int nc = a.wide || t.k1 - k >= KC ? KC : t.k1 - k, half = mma_n(t.rows) / 2;
+      // the leader's full[s] expects the bytes of both CTAs
+      if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * nc * (OP_BYTES + half * KB));
+      const uint32_t st = smem_u32(smem + s * STAGE_BYTES), fb = full_lead + 8 * s;
+      const int y = t.ch0 + 128 * (int)rank;
+      if (a.wide) {
+        tma_load_4d_pair(st, &maps.w, 0, y, k, t.group, fb);
+      } else {
         for (int c = 0; c < nc; ++c)
-          tma_load_3d_pair(st + c * OP_BYTES, &mw, (k + c) * KB, t.ch0 + 128 * (int)rank, t.group,
-                           full_lead + 8 * s);
-      };
-      auto load_t = [&](const Tile& t, int k, int s) {
-        const int nc = t.k1 - k < KC ? t.k1 - k : KC, half = mma_n(t.rows) / 2;
-        const int y = t.row0 + (int)rank * half;
-        const uint32_t fb = full_lead + 8 * s;
-        for (int c = 0; c < nc; ++c) {
-          const uint32_t sb = smem_u32(smem + s * STAGE_BYTES) + (KC + c) * OP_BYTES;
-          const int x = (k + c) * KB;
-          if (half == 128) {
-            tma_load_2d_pair(sb, &mt128, x, y, fb);
-          } else {
-            for (int i = 0; i < half; i += 32) tma_load_2d_pair(sb + i * KB, &mt32, x, y + i, fb);
-          }
-        }
-      };
-      bool ok = true, first = true;
-      for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
-        const Tile t = decode(a, table, w);
-        if (t.group == p.groups) continue;
-        int k = t.k0;
-        if (first) {
-          // the weight does not depend on the kernel before this one (the tokens'
-          // quantization): its first stages are on their way while that ends
-          for (; issued < STAGES && k < t.k1; k += KC) load_w(t, k, issued++);
-          wait_predecessor();
-          for (int s = 0, kk = t.k0; s < issued; ++s, kk += KC) load_t(t, kk, s);
-          first = false;
-        }
-        for (; k < t.k1; k += KC) {
-          const int s = issued % STAGES;
-          const uint32_t ph = (issued / STAGES) & 1;
-          ok = mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, a.wait_cycles);
-          if (!ok) break;
-          ++issued;
+          tma_load_4d_pair(st + c * OP_BYTES, &maps.w, (k + c) * KB, y, 0, t.group, fb);
+      }
+    };
+    auto load_t = [&](const Tile& t, int k, int s) {
+      const int nc = t.k1 - k < KC ? t.k1 - k : KC, half = mma_n(t.rows) / 2;
+      const int y = t.row0 + (int)rank * half;
+      const uint32_t sb = smem_u32(smem + s * STAGE_BYTES) + KC * OP_BYTES, fb = full_lead + 8 * s;
+      const CUtensorMap* m = &maps.t[half / 32 - 1];
+      if (a.wide) {
+        tma_load_3d_pair(sb, m, 0, y, k, fb);
+      } else {
+        for (int c = 0; c < nc; ++c) tma_load_3d_pair(sb + c * half * KB, m, (k + c) * KB, y, 0, fb);
+      }
+    };
+    bool ok = true, first = true;
+    for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
+      const Tile t = decode(a, table, w);
+      if (t.group == p.groups) continue;
+      int k = t.k0;
+      if (first) {
+        // the weight does not depend on the kernel before this one (the tokens'
+        // quantization): its first stages are on their way while that ends
+        for (; issued < STAGES && k < t.k1; k += KC, ++issued)
+          if (lane == 0) load_w(t, k, issued);
+        wait_predecessor();
+        for (int s = 0, kk = t.k0; s < issued; ++s, kk += KC)
+          if (lane == 0) load_t(t, kk, s);
+        first = false;
+      }
+      for (; k < t.k1; k += KC) {
+        const int s = issued % STAGES;
+        const uint32_t ph = (issued / STAGES) & 1;
+        ok = mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, a.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++issued;
+        if (lane == 0) {
           load_w(t, k, s);
           load_t(t, k, s);
         }
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       int it = 0, tc = 0;
       bool ok = true;
       for (int w = blockIdx.x >> 1; ok && w < total; w += step) {
@@ -313,30 +358,37 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t use_ph = (uint32_t)((tc >> 1) & 1);
         ++tc;
         ok = mbar_wait(acce0 + 8 * buf, use_ph ^ 1, abort_flag, p.status, a.wait_cycles);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
         const uint32_t acc = tmem + (uint32_t)(buf * TOK);
-        const uint32_t idesc = idesc_i8_m256(mma_n(t.rows));
+        const int n = mma_n(t.rows);
+        const uint32_t idesc = idesc_i8_m256(n);
         for (int k = t.k0; k < t.k1; k += KC) {
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1;
           ok = mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, a.wait_cycles);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           ++it;
           fence_after();
-          const int nc = t.k1 - k < KC ? t.k1 - k : KC;
-          const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
-          for (int c = 0; c < nc; ++c) {
-            const uint64_t da = desc_k_sw128(st + c * OP_BYTES);
-            const uint64_t db = desc_k_sw128(st + (KC + c) * OP_BYTES);
+          if (lane == 0) {
+            const int nc = t.k1 - k < KC ? t.k1 - k : KC;
+            const uint32_t st = smem_u32(smem + s * STAGE_BYTES);
+            for (int c = 0; c < nc; ++c) {
+              const uint64_t da = desc_k_sw128(st + c * OP_BYTES);
+              const uint64_t db = desc_k_sw128(st + KC * OP_BYTES + c * (n / 2) * KB);
 #pragma unroll
-            for (int kk = 0; kk < KB / 32; ++kk)  // 32 bytes of K per MMA
-              umma_i8_pair(acc, da + 2 * kk, db + 2 * kk, idesc,
-                           k > t.k0 || c > 0 || kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < KB / 32; ++kk)  // 32 bytes of K per MMA
+                umma_i8_pair(acc, da + 2 * kk, db + 2 * kk, idesc,
+                             k > t.k0 || c > 0 || kk > 0 ? 1u : 0u);
+            }
+            umma_commit_pair(empty0 + 8 * s);
           }
-          umma_commit_pair(empty0 + 8 * s);
+          __syncwarp();
         }
-        if (ok) umma_commit_pair(accf0 + 8 * buf);
+        if (ok && lane == 0) umma_commit_pair(accf0 + 8 * buf);
+        __syncwarp();
       }
     }
   } else {
@@ -519,11 +571,11 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 
 static bool byte_map(CUtensorMap* m, const void* base, int rank, const cuuint64_t* dims,
-                     const cuuint64_t* strides, int box_rows) {
+                     const cuuint64_t* strides, int box_rows, int box_chunks) {
   auto enc = encode_fn();
   if (!enc) return false;
-  const cuuint32_t box[3] = {KB, (cuuint32_t)box_rows, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
+  const cuuint32_t box[4] = {KB, (cuuint32_t)box_rows, (cuuint32_t)box_chunks, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
   return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(base), dims, strides, box,
              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -585,7 +637,7 @@ size_t tc_workspace_bytes(const Product& p) {
 }
 
 template <typename S>
-static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, bool overlap,
+static int launch_tc(const Maps& maps, const TcArgs& a, long long tiles, bool overlap,
                      cudaStream_t st) {
   const int smem = STAGES * STAGE_BYTES + 1024 + BAR_BYTES + EPI_WARPS * STRIP_BYTES +
                    2 * TOK * (int)sizeof(float) +
@@ -613,7 +665,7 @@ static int launch_tc(const CUtensorMap* maps, const TcArgs& a, long long tiles, 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = overlap ? 2 : 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, tc_kernel<S>, maps[0], maps[1], maps[2], a);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, tc_kernel<S>, maps, a);
   g2q::note_launch();
   if (e == cudaSuccess && a.splits > 1) {
     cudaLaunchConfig_t fin = {};
@@ -649,17 +701,32 @@ int tc_product(const Product& p, void* workspace, size_t workspace_bytes, bool o
   const size_t need = tc_workspace_bytes(p);
   if (need && (!workspace || workspace_bytes < need || !rows::aligned(workspace, 16)))
     return G2Q_ERR_INVALID_ARG;
-  const long long lda = p.M == 1 ? up16(p.K) : p.lda, ldb = p.N == 1 ? up16(p.K) : p.ldb;
-  const cuuint64_t wd[3] = {(cuuint64_t)p.K, (cuuint64_t)p.N, (cuuint64_t)p.groups};
-  const cuuint64_t ws[2] = {(cuuint64_t)ldb, (cuuint64_t)(p.groups > 1 ? p.b_gs : p.N * ldb)};
-  const cuuint64_t td[2] = {(cuuint64_t)p.K, (cuuint64_t)p.M};
-  const cuuint64_t ts[1] = {(cuuint64_t)lda};
-  CUtensorMap maps[3];
-  if (!byte_map(&maps[0], p.b, 3, wd, ws, 128) || !byte_map(&maps[1], p.a, 2, td, ts, 128) ||
-      !byte_map(&maps[2], p.a, 2, td, ts, 32))
-    return G2Q_ERR_CUDA;
+  a.wide = p.K % KB == 0;
+  a.per_band = 1.f / (float)(RASTER * a.ch_tiles);
+  const cuuint64_t lda = (cuuint64_t)(p.M == 1 ? up16(p.K) : p.lda);
+  const cuuint64_t ldb = (cuuint64_t)(p.N == 1 ? up16(p.K) : p.ldb);
+  const cuuint64_t gs = p.groups > 1 ? (cuuint64_t)p.b_gs : (cuuint64_t)p.N * ldb;
+  const cuuint64_t inner = (cuuint64_t)(a.wide ? KB : p.K), chunks = (cuuint64_t)(a.wide ? a.nk : 1);
+  const cuuint64_t wd[4] = {inner, (cuuint64_t)p.N, chunks, (cuuint64_t)p.groups};
+  const cuuint64_t ws[3] = {ldb, KB, gs};
+  const cuuint64_t td[3] = {inner, (cuuint64_t)p.M, chunks};
+  const cuuint64_t ts[2] = {lda, KB};
+  const int box_chunks = a.wide ? KC : 1;
+  Maps maps;
+  if (!byte_map(&maps.w, p.b, 4, wd, ws, 128, box_chunks)) return G2Q_ERR_CUDA;
+  // the heights that occur: one group has whole pieces and a last one
+  const int whole = a.tok / 2, last = (int)((p.M % a.tok + 63) / 64 * 32);
+  for (int i = 0; i < 4; ++i) {
+    const int rows = 32 * (i + 1);
+    if (p.offsets ? rows <= whole : ((rows == whole && p.M >= a.tok) || rows == last)) {
+      if (!byte_map(&maps.t[i], p.a, 3, td, ts, rows, box_chunks)) return G2Q_ERR_CUDA;
+    } else {
+      maps.t[i] = maps.w;  // never read
+    }
+  }
   const long long tiles = range_slots(p, a.tok) * a.ch_tiles * a.splits;
-  if (tiles > 0x3fffffffLL) return G2Q_ERR_UNSUPPORTED;
+  // (tile numbers also have to be exact in fp32 to within one band)
+  if (tiles > 0xffffffLL) return G2Q_ERR_UNSUPPORTED;
   if (p.out_dtype == G2Q_DTYPE_BF16) return launch_tc<__nv_bfloat16>(maps, a, tiles, overlap, st);
   if (p.out_dtype == G2Q_DTYPE_F16) return launch_tc<__half>(maps, a, tiles, overlap, st);
   return launch_tc<float>(maps, a, tiles, overlap, st);
