@@ -248,6 +248,33 @@ def test_int8_matmul(dtype, M, N, K):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(9001, 5016, 2048), (8500, 5001, 2064), (9472, 4864, 2176)])
+def test_int8_matmul_large(dtype, M, N, K):
+    """Sizes at which the largest tiles are chosen, rows ending in each of a tile's
+    blocks."""
+    g = gen(M)
+    a, b = aligned_codes((M, K), g), aligned_codes((N, K), g)
+    sa, sb = torch.rand(M, generator=g, device=DEV), torch.rand(N, generator=g, device=DEV)
+    check_product(ops.int8_matmul(a, sa, b, sb, out_dtype=dtype), a, sa, b, sb, None)
+
+
+@gpu
+@pytest.mark.parametrize("K", [2048, 2064])
+@pytest.mark.parametrize("counts,tail", [([1100, 0, 613], 5), ([512, 1024, 257, 300], 0),
+                                         ([3, 2000, 10], 700)])
+def test_int8_matmul_grouped_large(counts, tail, K):
+    a, sa, b, sb, off = grouped_case(counts, tail, 520, K, tail)
+    got = ops.int8_matmul_grouped(a, sa, b, sb, off)
+    cut = off.tolist()
+    for e in range(len(counts)):
+        lo, hi = cut[e], cut[e + 1]
+        if hi > lo:
+            check_product(got[lo:hi], a[lo:hi], sa[lo:hi], b[e], sb[e], None)
+    assert not bool(got[cut[-1]:].any())
+
+
+@gpu
 @pytest.mark.parametrize("M,N,K,pa,pb", [(5, 70, 33, 0, 0), (70, 65, 130, 3, 1), (3, 9, 4, 0, 5),
                                          (130, 140, 63, 1, 0)])
 def test_int8_matmul_unaligned_rows(M, N, K, pa, pb):
