@@ -23,7 +23,6 @@ using rows::of_f;
 
 constexpr int SW = 8;       // warps per CTA
 constexpr int STEP = 64;    // bytes of K per warp and step
-constexpr int DEPTH = 4;    // steps whose loads are in flight together
 
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                        uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -34,9 +33,14 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Bytes k .. k + 15 of a row of K bytes, missing ones zero.
+// Bytes k .. k + 15 of a row of K bytes, missing ones zero.  ONCE: read a single
+// time (the weight), so not kept (23.5 -> 20.8 us for four tokens' 128 experts).
+template <bool ONCE>
 __device__ __forceinline__ uint4 load16(const int8_t* row, long long k, long long K) {
-  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  if (k + 16 <= K) {
+    const uint4* v = reinterpret_cast<const uint4*>(row + k);
+    return ONCE ? __ldcs(v) : __ldg(v);
+  }
   uint32_t w[4] = {0, 0, 0, 0};
   if (k < K) {
 #pragma unroll
@@ -88,6 +92,9 @@ struct Input {  // the tokens before quantization (FUSED)
 template <typename S, typename X, int RG, int MG, bool FUSED>
 __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const Input in) {
   constexpr int KS = SW / RG, TOKENS = 8 * MG, CHANNELS = 16 * RG;
+  // steps whose loads are in flight together (eight instead of four: 5.3 -> 5.0 us
+  // for eight tokens through 4096 x 4096; with more channels per CTA slower)
+  constexpr int DEPTH = RG == 1 && MG == 1 ? 8 : 4;
   extern __shared__ uint4 dyn[];  // FUSED: codes [M][pitch]
   __shared__ int red[KS][CHANNELS][TOKENS + 1];
   __shared__ float sa_s[TOKENS];
@@ -121,8 +128,8 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
       const long long k = ((long long)turn * DEPTH + d) * STEP + 16 * t4;
-      wa[d] = load16(w0, k, p.K);
-      wb[d] = load16(w1, k, p.K);
+      wa[d] = load16<true>(w0, k, p.K);
+      wb[d] = load16<true>(w1, k, p.K);
     }
   };
   load_w(ks);
@@ -160,7 +167,7 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
           tok[d][j] = make_uint4(0, 0, 0, 0);
           if (m < have && k < p.K) {
             if (FUSED) tok[d][j] = *reinterpret_cast<const uint4*>(codes + (long long)m * pitch + k);
-            else tok[d][j] = load16(p.a + (m0 + m) * p.lda, k, p.K);
+            else tok[d][j] = load16<false>(p.a + (m0 + m) * p.lda, k, p.K);
           }
         }
       }
@@ -256,12 +263,20 @@ int stream_product(const Product& p, bool overlap, cudaStream_t st) {
   return stream_out<float>(p, overlap, st);
 }
 
+template <typename S, typename X>
+static int stream_in_out(const Product& p, const Input& in, cudaStream_t st) {
+  // more CTAs than are resident at once: half as many, which quantize the token
+  // half as often (14336 x 4096 13.8 us, with 16 channels per CTA 17.1 us; 4096 x
+  // 4096 5.7 and 4.6 us)
+  if (p.N > 148 * 3 * 16) return launch_stream<S, X, 2, 1, true>(p, in, false, st);
+  return launch_stream<S, X, 1, 1, true>(p, in, false, st);
+}
+
 template <typename X>
 static int stream_in(const Product& p, const Input& in, cudaStream_t st) {
-  if (p.out_dtype == G2Q_DTYPE_BF16)
-    return launch_stream<__nv_bfloat16, X, 1, 1, true>(p, in, false, st);
-  if (p.out_dtype == G2Q_DTYPE_F16) return launch_stream<__half, X, 1, 1, true>(p, in, false, st);
-  return launch_stream<float, X, 1, 1, true>(p, in, false, st);
+  if (p.out_dtype == G2Q_DTYPE_BF16) return stream_in_out<__nv_bfloat16, X>(p, in, st);
+  if (p.out_dtype == G2Q_DTYPE_F16) return stream_in_out<__half, X>(p, in, st);
+  return stream_in_out<float, X>(p, in, st);
 }
 
 int stream_linear(const Product& p, const void* x, int x_dtype, long long ldx, cudaStream_t st) {
