@@ -568,6 +568,7 @@ def make_moe(torch, dev, rank, world, args):
     the down projections' inputs (BF16 N(0, 1), the stand-in for
     act(gate) * up).  Made outside the timed region, like the Llama
     workload's activations."""
+    from g2ptq_b200.utils import moe_utils
     g = torch.Generator(device=dev).manual_seed(42)
     experts = {}
     for proj, (rows, cols) in (("gate_proj", (MOE_INTER, MOE_HIDDEN)),
@@ -588,16 +589,13 @@ def make_moe(torch, dev, rank, world, args):
         x = torch.randn(n * args.seq_len, MOE_HIDDEN, device=dev, generator=gx)
         x[:, idx_out] *= 20.0
         x = x.to(torch.bfloat16)
-        top = torch.topk(x.float() @ router.T, MOE_TOPK, dim=-1).indices.reshape(-1)
-        order = torch.argsort(top, stable=True)
-        counts = torch.bincount(top, minlength=MOE_EXPERTS).tolist()
-        routed = x[order // MOE_TOPK].contiguous()
+        top = torch.topk(x.float() @ router.T, MOE_TOPK, dim=-1).indices
+        routing = moe_utils.route(top, MOE_EXPERTS)
+        routed = moe_utils.dispatch(x, routing)
         down_in = torch.randn(routed.shape[0], MOE_INTER, device=dev, generator=gx).to(
             torch.bfloat16)
-        bounds, c0 = [], 0
-        for c in counts:
-            bounds.append((c0, c0 + c))
-            c0 += c
+        cut = routing.offsets.tolist()
+        bounds = list(zip(cut, cut[1:]))
         batches.append((routed, down_in, bounds))
     return experts, batches
 

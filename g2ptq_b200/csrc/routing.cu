@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(256)
 // Loads in flight are what counts: with eight slots, registers for six CTAs per SM
 // instead of four took 184 us for 204 us (16384 x 8 rows of 2048 bf16).
 template <typename S, int W, int KT, int U, int WARPS>
-__global__ void __launch_bounds__(128, KT == 8 && U == 1 ? 6 : 4)
+__global__ void __launch_bounds__(128, KT == 8 ? (U == 1 ? 6 : 3) : 4)
     combine_bwd_kernel(S* __restrict__ gy, long long ldgy, void* __restrict__ gw,
                        const S* __restrict__ g, long long ldg, const S* __restrict__ y,
                        long long ldy, const int32_t* __restrict__ position,

@@ -9,6 +9,12 @@
     python kernel_cases.py block_loss --tokens 2048 --vocab 128256 --loss kl
     python kernel_cases.py saliency --tokens 8192 --rows 14336
     python kernel_cases.py running_mean --rows 14336 --columns 4096
+    python kernel_cases.py quantize_tokens --tokens 16384 --columns 4096
+    python kernel_cases.py int8_linear --tokens 16384 --rows 14336 --columns 4096
+    python kernel_cases.py int8_experts --tokens 8192 --rows 2048 --columns 768
+    python kernel_cases.py route --tokens 65536
+    python kernel_cases.py dispatch --tokens 65536 --columns 2048
+    python kernel_cases.py combine --tokens 16384 --columns 2048
 
 Each case builds seeded synthetic inputs of one fold / one factorization /
 one compensation pass of a Llama-3-8B linear on ``cuda:0``, runs ``--warmup``
@@ -24,6 +30,7 @@ import json
 import torch
 
 from g2ptq_b200 import ops, _lib
+from g2ptq_b200.utils import moe_utils
 
 
 def _time(fn, warmup, reps):
@@ -274,10 +281,89 @@ def running_mean(args, g):
     return dict(case="running_mean", rows=R, columns=C, ms=ms, bytes=b, gbs=b / ms / 1e6)
 
 
+def _routing(args, g):
+    """Top-``topk`` of ``experts`` random logits per token."""
+    T = args.tokens or 16384
+    ids = torch.topk(torch.randn(T, args.experts, device="cuda", generator=g), args.topk,
+                     dim=-1).indices
+    return T, T * args.topk, ids, moe_utils.route(ids, args.experts)
+
+
+def _codes(shape, g):
+    return torch.randint(-128, 128, shape, device="cuda", generator=g, dtype=torch.int8)
+
+
+def quantize_tokens(args, g):
+    """int8 codes and scales of ``tokens`` x ``columns`` BF16 activations."""
+    T, C = args.tokens or 16384, args.columns
+    x = torch.randn(T, C, device="cuda", generator=g).to(torch.bfloat16)
+    ms = _time(lambda: ops.quantize_tokens(x), args.warmup, args.reps)
+    b = T * C * 3 + 4 * T
+    return dict(case="quantize_tokens", tokens=T, columns=C, ms=ms, bytes=b, gbs=b / ms / 1e6)
+
+
+def int8_linear(args, g):
+    """``tokens`` x ``columns`` BF16 through a ``rows`` x ``columns`` 8-bit linear."""
+    T, R, C = args.tokens or 16384, args.rows, args.columns
+    x = torch.randn(T, C, device="cuda", generator=g).to(torch.bfloat16)
+    w, s = _codes((R, C), g), torch.ones(R, device="cuda")
+    ms = _time(lambda: ops.int8_linear(x, w, s), args.warmup, args.reps)
+    b = T * C * 2 + R * C + T * R * 2
+    return dict(case="int8_linear", tokens=T, rows=R, columns=C, ms=ms, bytes=b,
+                gbs=b / ms / 1e6, tops=2 * T * R * C / ms / 1e9)
+
+
+def int8_experts(args, g):
+    """The routed rows of ``tokens`` through the experts' 8-bit linears."""
+    R, C = args.rows, args.columns
+    T, n, _, routing = _routing(args, g)
+    x = torch.randn(n, C, device="cuda", generator=g).to(torch.bfloat16)
+    w, s = _codes((args.experts, R, C), g), torch.ones(args.experts, R, device="cuda")
+    ms = _time(lambda: ops.int8_linear_grouped(x, w, s, routing.offsets), args.warmup, args.reps)
+    b = n * C * 2 + args.experts * R * C + n * R * 2
+    return dict(case="int8_experts", tokens=T, routed_rows=n, rows=R, columns=C, ms=ms, bytes=b,
+                gbs=b / ms / 1e6, tops=2 * n * R * C / ms / 1e9)
+
+
+def route(args, g):
+    """The (token, slot) pairs of ``tokens`` sorted by expert."""
+    T, n, ids, _ = _routing(args, g)
+    ms = _time(lambda: moe_utils.route(ids, args.experts), args.warmup, args.reps)
+    b = n * 16 + 4 * args.experts
+    return dict(case="route", tokens=T, ms=ms, bytes=b, gbs=b / ms / 1e6)
+
+
+def dispatch(args, g):
+    """``tokens`` x ``columns`` BF16 rows copied into expert order."""
+    C = args.columns
+    T, n, _, routing = _routing(args, g)
+    x = torch.randn(T, C, device="cuda", generator=g).to(torch.bfloat16)
+    ms = _time(lambda: moe_utils.dispatch(x, routing), args.warmup, args.reps)
+    b = (T + n) * C * 2
+    return dict(case="dispatch", tokens=T, columns=C, ms=ms, bytes=b, gbs=b / ms / 1e6)
+
+
+def combine(args, g):
+    """The routed rows back in token order, weighted, and both gradients."""
+    C = args.columns
+    T, n, _, routing = _routing(args, g)
+    y = torch.randn(n, C, device="cuda", generator=g).to(torch.bfloat16)
+    w = torch.rand(T, args.topk, device="cuda", generator=g)
+    out = moe_utils.combine(y, routing, w)
+    fwd = _time(lambda: moe_utils.combine(y, routing, w), args.warmup, args.reps)
+    bwd = _time(lambda: ops.combine_rows_backward(out, y, routing.position, w), args.warmup,
+                args.reps)
+    fb, bb = (n + T) * C * 2, (2 * n + T) * C * 2
+    return dict(case="combine", tokens=T, columns=C, fwd_ms=fwd, bwd_ms=bwd, fwd_bytes=fb,
+                bwd_bytes=bb, fwd_gbs=fb / fwd / 1e6, bwd_gbs=bb / bwd / 1e6)
+
+
 CASES = {"gram": gram, "gram_weighted": gram_weighted, "gram_grouped": gram_grouped,
          "chol": chol,
          "compensate": compensate, "block_loss": block_loss, "saliency": saliency,
-         "running_mean": running_mean, "sweep": sweep}
+         "running_mean": running_mean, "sweep": sweep, "quantize_tokens": quantize_tokens,
+         "int8_linear": int8_linear, "int8_experts": int8_experts, "route": route,
+         "dispatch": dispatch, "combine": combine}
 
 
 def main(argv=None):
@@ -293,6 +379,8 @@ def main(argv=None):
     ap.add_argument("--batch", type=int, default=1)
     ap.add_argument("--bits", type=int, default=4)
     ap.add_argument("--groupsize", type=int, default=128)
+    ap.add_argument("--experts", type=int, default=128)
+    ap.add_argument("--topk", type=int, default=8)
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--reps", type=int, default=5)
     args = ap.parse_args(argv)
