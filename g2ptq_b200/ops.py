@@ -567,8 +567,14 @@ def _call_on(idx, name, *args):
 
 
 def _status_word(idx):
+    """The device's status word; None (discard) in a graph capture that would have
+    to make it, whose zeros only a replay would write."""
     t = _DEVICE_STATUS.get(idx)
-    return (device_status(torch.device("cuda", idx)) if t is None else t).data_ptr()
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        t = device_status(torch.device("cuda", idx))
+    return t.data_ptr()
 
 
 def _rows_bytes(nbytes, like):

@@ -102,8 +102,8 @@ def routed_experts_forward(experts, hidden, top_experts, top_weights):
     rows = dispatch(hidden, routing)
     cut = routing.offsets.tolist()
     parts = [experts[e](rows[a:b]) for e, (a, b) in enumerate(zip(cut, cut[1:])) if b > a]
-    if not parts:
-        return torch.zeros_like(hidden)
+    if not parts:  # zeros, and zero gradients
+        return combine(rows, routing, top_weights)
     tail = rows.shape[0] - cut[-1]
     if tail:
         parts.append(parts[0].new_zeros(tail, parts[0].shape[1]))

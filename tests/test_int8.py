@@ -525,6 +525,28 @@ def test_side_stream_and_graph():
 
 
 @gpu
+def test_capture_without_a_status_word():
+    """A first call inside a capture makes no status word there: its zeros would be
+    written by a replay only."""
+    g = gen(8)
+    codes, scale = aligned_codes((64, 128), g), torch.rand(64, generator=g, device=DEV)
+    x = torch.randn(300, 128, generator=g, device=DEV)
+    want = int8_utils.int8_linear(x, codes, scale)  # loads the library
+    words = dict(ops._DEVICE_STATUS)
+    ops._DEVICE_STATUS.clear()
+    try:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            y = int8_utils.int8_linear(x, codes, scale)
+        assert not ops._DEVICE_STATUS
+    finally:
+        ops._DEVICE_STATUS.update(words)
+    gr.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+
+
+@gpu
 def test_moe_layer_in_8_bits():
     """Router, sort, gate / up and down of every expert in 8 bits and the weighted
     way back, against the same steps in 64 bits on the same codes."""

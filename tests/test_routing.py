@@ -373,10 +373,12 @@ def test_routed_experts_forward():
 def test_no_token_has_an_expert():
     g = gen(14)
     experts = [Expert(8, 8, torch.float32, g)]
-    x = torch.randn(4, 8, generator=g, device=DEV)
-    out = moe_utils.routed_experts_forward(experts, x, torch.full((4, 2), -1, device=DEV),
-                                           torch.ones(4, 2, device=DEV))
-    assert not bool(out.any())
+    x = torch.randn(4, 8, generator=g, device=DEV).requires_grad_()
+    w = torch.ones(4, 2, device=DEV).requires_grad_()
+    out = moe_utils.routed_experts_forward(experts, x, torch.full((4, 2), -1, device=DEV), w)
+    assert out.shape == x.shape and not bool(out.any())
+    gx, gw = torch.autograd.grad(out.sum(), (x, w))
+    assert not bool(gx.any()) and not bool(gw.any())
 
 
 @gpu
