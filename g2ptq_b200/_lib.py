@@ -152,6 +152,38 @@ def load():
     return lib
 
 
+# what the native binding calls
+_BOUND = ("g2q_quantize_tokens", "g2q_int8_matmul", "g2q_int8_matmul_workspace_bytes",
+          "g2q_int8_matmul_grouped", "g2q_int8_linear", "g2q_int8_linear_workspace_bytes",
+          "g2q_route", "g2q_route_workspace_bytes", "g2q_dispatch_rows", "g2q_combine_rows",
+          "g2q_combine_rows_backward")
+_binding = None
+
+
+def binding():
+    """The native torch binding (csrc/binding.cpp) of the operators called token by
+    token, bound to the loaded library; raises OSError when it is not built."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    path = os.path.join(_HERE, "_lib", "_binding.so")
+    if not os.path.exists(path):
+        raise OSError(f"g2ptq_b200 torch binding not found at {path}; build it with "
+                      "`python -m g2ptq_b200.build`")
+    import importlib.util
+
+    import torch  # noqa: F401  (its libraries have to be loaded first)
+    from . import ops
+    lib = load()
+    spec = importlib.util.spec_from_file_location("_binding", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.bind({n: ctypes.cast(getattr(lib, n), P).value for n in _BOUND}, G2QError,
+             lambda idx: ops.status_word(idx) or 0)
+    _binding = mod
+    return mod
+
+
 def status_string(status):
     return load().g2q_status_string(int(status)).decode()
 

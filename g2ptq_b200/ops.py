@@ -539,70 +539,24 @@ def block_loss_backward(kind, stats, x2, t2, labels, grad_scale=None):
 
 # --------------------------------------------------------------------------
 # 8-bit linears: per-token int8 activations and the scaled integer product
+#
+# These and the routing below are called token by token, so checks, allocation and
+# the call are one step in the native binding (csrc/binding.cpp).
 # --------------------------------------------------------------------------
 
 INT8_MAX_K = 131071  # |a b| <= 128 * 128: longer sums could leave 32 bits
 MAX_EXPERTS = 1024
 
 
-def _device_of(*tensors):
-    """Index of the CUDA device that every given tensor (None: skipped) is on;
-    ``_cuda``'s errors."""
-    idx = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and (idx < 0 or t.get_device() != idx):
-            _cuda(*tensors)
-    return idx
-
-
-def _call_on(idx, name, *args):
-    """``call`` with device ``idx`` current and its current stream as the last
-    argument: a kernel is launched on the current device, which need not be the
-    tensors'."""
-    stream = torch._C._cuda_getCurrentRawStream(idx)
-    if torch.cuda.current_device() == idx:
-        return call(name, *args, stream)
-    with torch.cuda.device(idx):
-        return call(name, *args, stream)
-
-
-def _status_word(idx):
-    """The device's status word; None (discard) in a graph capture that would have
-    to make it, whose zeros only a replay would write."""
+def status_word(idx):
+    """Address of device ``idx``'s status word; None (discard) in a graph capture
+    that would have to make it, whose zeros only a replay would write."""
     t = _DEVICE_STATUS.get(idx)
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             return None
         t = device_status(torch.device("cuda", idx))
     return t.data_ptr()
-
-
-def _rows_bytes(nbytes, like):
-    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-
-
-def _matrix(name, t):
-    """``(rows, columns, row stride)`` of the 2-D ``t`` with unit column stride and
-    rows that do not overlap."""
-    if t.dim() != 2:
-        raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
-    rows, cols = t.shape
-    ld, step = t.stride()
-    if cols > 1 and step != 1:
-        raise ValueError(f"{name} needs unit column stride")
-    if rows <= 1:
-        return rows, cols, max(cols, 1)
-    if ld < cols:
-        raise ValueError(f"{name} has overlapping rows")
-    return rows, cols, ld
-
-
-def _vector(name, t, n, dtype=torch.float32):
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n:
-        raise ValueError(f"{name} must be {dtype} of shape ({n},), got {t.dtype} of shape "
-                         f"{tuple(t.shape)}")
-    if n > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous")
 
 
 def int8_row_stride(cols):
@@ -617,79 +571,14 @@ def quantize_tokens(x):
     even.  A row whose values are all zero has scale 1; one with an infinity or
     a NaN has scale NaN and codes 0.  Returns ``(codes [T, C], scale [T])``, the
     codes' rows ``int8_row_stride(C)`` apart."""
-    idx = _device_of(x)
-    T, C, ldx = _matrix("x", x)
-    if C == 0:
-        raise ValueError("quantize_tokens needs at least one column")
-    dt = dtype_code(x.dtype)
-    ldq = int8_row_stride(C)
-    codes = x.new_empty((T, ldq), dtype=torch.int8)[:, :C]
-    scale = x.new_empty(T, dtype=torch.float32)
-    _call_on(idx, "g2q_quantize_tokens", codes.data_ptr(), ldq, scale.data_ptr(), x.data_ptr(), dt,
-             ldx, T, C)
-    return codes, scale
-
-
-def _weight(b, b_scale, K):
-    """``(N, ldb)`` of int8 codes ``b [N, K]`` with their scales."""
-    if b.dtype != torch.int8:
-        raise TypeError(f"the weight must be int8 codes, got {b.dtype}")
-    N, Kb, ldb = _matrix("b", b)
-    if Kb != K:
-        raise ValueError(f"the tokens have {K} columns and the weight {Kb}")
-    if not 0 < K <= INT8_MAX_K or N == 0:
-        raise ValueError(f"needs 1 to {INT8_MAX_K} columns and at least one channel")
-    _vector("b_scale", b_scale, N)
-    return N, ldb
-
-
-def _expert_weight(b, b_scale, offsets, K):
-    """``(E, N, ldb, b_gs)`` of the stacked codes ``b [E, N, K]``."""
-    if b.dtype != torch.int8:
-        raise TypeError(f"the weight must be int8 codes, got {b.dtype}")
-    if b.dim() != 3:
-        raise ValueError(f"b must be [experts, channels, columns], got shape {tuple(b.shape)}")
-    E, N, Kb = b.shape
-    if Kb != K:
-        raise ValueError(f"the rows have {K} columns and the weight {Kb}")
-    if not 0 < K <= INT8_MAX_K or N == 0 or not 0 < E <= MAX_EXPERTS:
-        raise ValueError(f"needs 1 to {INT8_MAX_K} columns, at least one channel and 1 to "
-                         f"{MAX_EXPERTS} experts")
-    gs, ld, step = b.stride()
-    ldb = ld if N > 1 else K
-    if (K > 1 and step != 1) or ldb < K or (E > 1 and gs < N * ldb):
-        raise ValueError("b needs unit column stride and experts and rows that do not overlap")
-    if b_scale.dtype != torch.float32 or b_scale.shape != (E, N) or not b_scale.is_contiguous():
-        raise ValueError(f"b_scale must be contiguous fp32 of shape ({E}, {N})")
-    _vector("offsets", offsets, E + 1, torch.int32)
-    return E, N, ldb, gs if E > 1 else N * ldb
-
-
-def _codes(a, a_scale):
-    if a.dtype != torch.int8:
-        raise TypeError(f"the tokens must be int8 codes, got {a.dtype}")
-    M, K, lda = _matrix("a", a)
-    _vector("a_scale", a_scale, M)
-    return M, K, lda
+    return _lib.binding().quantize_tokens(x)
 
 
 def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
     """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k] + bias[n]``
     for int8 ``a [M, K]`` and ``b [N, K]``, fp32 scales and bias; the sums are
     exact.  Rows 16 bytes aligned (``int8_row_stride``) run on the tensor cores."""
-    idx = _device_of(a, a_scale, b, b_scale, bias)
-    M, K, lda = _codes(a, a_scale)
-    N, ldb = _weight(b, b_scale, K)
-    if bias is not None:
-        _vector("bias", bias, N)
-    dt = dtype_code(out_dtype)
-    out = a.new_empty((M, N), dtype=out_dtype)
-    ws_bytes = query("g2q_int8_matmul_workspace_bytes", M, N, K)
-    ws = _rows_bytes(ws_bytes, a)
-    _call_on(idx, "g2q_int8_matmul", out.data_ptr(), dt, N, a.data_ptr(), lda, a_scale.data_ptr(),
-             b.data_ptr(), ldb, b_scale.data_ptr(), _ptr(bias), M, N, K, _ptr(ws), ws_bytes,
-             _status_word(idx))
-    return out
+    return _lib.binding().int8_matmul(a, a_scale, b, b_scale, bias, out_dtype)
 
 
 def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat16):
@@ -697,50 +586,19 @@ def int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype=torch.bfloat1
     ``offsets[e + 1] - 1`` of ``a [R, K]`` are multiplied with ``b[e]`` of
     ``b [E, N, K]`` and scaled by ``b_scale [E, N]``.  ``offsets`` is int32
     ``[E + 1]``, ascending from 0; rows behind ``offsets[E]`` give zeros."""
-    idx = _device_of(a, a_scale, b, b_scale, offsets)
-    R, K, lda = _codes(a, a_scale)
-    E, N, ldb, b_gs = _expert_weight(b, b_scale, offsets, K)
-    dt = dtype_code(out_dtype)
-    out = a.new_empty((R, N), dtype=out_dtype)
-    _call_on(idx, "g2q_int8_matmul_grouped", out.data_ptr(), dt, N, a.data_ptr(), lda,
-             a_scale.data_ptr(), b.data_ptr(), ldb, b_gs, b_scale.data_ptr(), offsets.data_ptr(),
-             E, R, N, K, _status_word(idx))
-    return out
+    return _lib.binding().int8_matmul_grouped(a, a_scale, b, b_scale, offsets, out_dtype)
 
 
 def int8_linear(x, codes, scale, bias=None):
     """``quantize_tokens`` of ``x [M, K]`` and ``int8_matmul`` with ``codes [N, K]``
     in one call; the result has ``x``'s type."""
-    idx = _device_of(x, codes, scale, bias)
-    M, K, ldx = _matrix("x", x)
-    N, ldb = _weight(codes, scale, K)
-    if bias is not None:
-        _vector("bias", bias, N)
-    dt = dtype_code(x.dtype)
-    out = x.new_empty((M, N))
-    b = codes.data_ptr()
-    ws_bytes = query("g2q_int8_linear_workspace_bytes", M, N, K, 0, (b | ldb) % 16 == 0)
-    ws = _rows_bytes(ws_bytes, x)
-    _call_on(idx, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx, b, ldb, 0,
-             scale.data_ptr(), _ptr(bias), None, 0, M, N, K, _ptr(ws), ws_bytes, _status_word(idx))
-    return out
+    return _lib.binding().int8_linear(x, codes, scale, bias)
 
 
 def int8_linear_grouped(x, codes, scale, offsets):
     """``quantize_tokens`` of ``x [R, K]`` and ``int8_matmul_grouped`` with ``codes
     [E, N, K]`` in one call; the result has ``x``'s type."""
-    idx = _device_of(x, codes, scale, offsets)
-    R, K, ldx = _matrix("x", x)
-    E, N, ldb, b_gs = _expert_weight(codes, scale, offsets, K)
-    dt = dtype_code(x.dtype)
-    out = x.new_empty((R, N))
-    b = codes.data_ptr()
-    ws_bytes = query("g2q_int8_linear_workspace_bytes", R, N, K, E, (b | ldb | b_gs) % 16 == 0)
-    ws = _rows_bytes(ws_bytes, x)
-    _call_on(idx, "g2q_int8_linear", out.data_ptr(), dt, N, x.data_ptr(), dt, ldx, b, ldb, b_gs,
-             scale.data_ptr(), None, offsets.data_ptr(), E, R, N, K, _ptr(ws), ws_bytes,
-             _status_word(idx))
-    return out
+    return _lib.binding().int8_linear_grouped(x, codes, scale, offsets)
 
 
 # --------------------------------------------------------------------------
@@ -754,77 +612,23 @@ def route(experts, num_experts):
     ``t k + j`` in expert order, every pair's row there, and each expert's first
     row.  Pairs whose id is not in ``[0, num_experts)`` come last and have
     position ``-1 - row``."""
-    idx = _device_of(experts)
-    if experts.dim() != 2 or experts.shape[1] == 0:
-        raise ValueError(f"experts must be [tokens, slots], got shape {tuple(experts.shape)}")
-    wide = experts.dtype == torch.int64
-    if not wide and experts.dtype != torch.int32:
-        raise TypeError(f"experts must be int32 or int64, got {experts.dtype}")
-    if not 0 < num_experts <= MAX_EXPERTS:
-        raise ValueError(f"1 to {MAX_EXPERTS} experts, got {num_experts}")
-    _contig(experts)
-    n = experts.numel()
-    order = experts.new_empty(n, dtype=torch.int32)
-    position = experts.new_empty(experts.shape, dtype=torch.int32)
-    offsets = experts.new_empty(num_experts + 1, dtype=torch.int32)
-    ws_bytes = query("g2q_route_workspace_bytes", n, num_experts)
-    ws = _rows_bytes(ws_bytes, experts)
-    _call_on(idx, "g2q_route", order.data_ptr(), position.data_ptr(), offsets.data_ptr(),
-             experts.data_ptr(), wide, n, num_experts, _ptr(ws), ws_bytes)
-    return order, position, offsets
-
-
-def _positions(position):
-    if position.dtype != torch.int32 or position.dim() != 2 or position.shape[1] == 0:
-        raise ValueError("position must be int32 [tokens, slots]")
-    if not position.is_contiguous():
-        raise ValueError("position must be contiguous")
-    return position.shape
-
-
-def _weights(weights, position):
-    """dtype code of the routing weights (0 for None)."""
-    if weights is None:
-        return 0
-    if weights.shape != position.shape:
-        raise ValueError(f"weights must have shape {tuple(position.shape)}")
-    if not weights.is_contiguous():
-        raise ValueError("weights must be contiguous")
-    return dtype_code(weights.dtype)
+    return _lib.binding().route(experts, num_experts)
 
 
 def dispatch_rows(x, position):
     """Rows of ``x [T, C]`` (1-, 2- or 4-byte elements) copied to the rows that
     ``position [T, k]`` (of ``route``) gives each slot: ``[T k, C]``.  Rows of
-    pairs without an expert are zero."""
-    idx = _device_of(x, position)
-    T, k = _positions(position)
-    rows, C, ldx = _matrix("x", x)
-    if rows != T or C == 0:
-        raise ValueError(f"x must have {T} rows and at least one column")
-    if x.element_size() not in (1, 2, 4):
-        raise TypeError(f"unsupported dtype {x.dtype}")
-    out = x.new_empty((T * k, C))
-    _call_on(idx, "g2q_dispatch_rows", out.data_ptr(), C, x.data_ptr(), ldx, x.element_size(),
-             position.data_ptr(), T, k, C)
-    return out
+    pairs without an expert are zero.  No gradient (``moe_utils.dispatch``)."""
+    return _lib.binding().dispatch_rows(x, position)
 
 
 def combine_rows(y, position, weights=None):
     """``out[t] = sum_j weights[t, j] * y[position[t, j]]`` over the slots with an
     expert, added in slot order in fp32 and rounded once to ``y``'s type:
     ``y [T k, C]``, ``position [T, k]`` of ``route``, ``weights [T, k]`` (None:
-    ones).  A token without any expert gives zeros."""
-    idx = _device_of(y, position, weights)
-    T, k = _positions(position)
-    rows, C, ldy = _matrix("y", y)
-    if rows != T * k or C == 0:
-        raise ValueError(f"y must have {T * k} rows and at least one column")
-    dt, wdt = dtype_code(y.dtype), _weights(weights, position)
-    out = y.new_empty((T, C))
-    _call_on(idx, "g2q_combine_rows", out.data_ptr(), C, y.data_ptr(), ldy, dt,
-             position.data_ptr(), _ptr(weights), wdt, T, k, C)
-    return out
+    ones).  A token without any expert gives zeros.  No gradient
+    (``moe_utils.combine``)."""
+    return _lib.binding().combine_rows(y, position, weights)
 
 
 def combine_rows_backward(grad, y, position, weights, need_y=True, need_weights=True):
@@ -832,22 +636,4 @@ def combine_rows_backward(grad, y, position, weights, need_y=True, need_weights=
     ``(grad_y [T k, C], grad_weights [T, k])``, None for what is not needed (``y`` is
     read for the weights' gradient alone).  Rows and weights of pairs without an
     expert get zero."""
-    y = y if need_weights else None
-    idx = _device_of(grad, y, position, weights)
-    T, k = _positions(position)
-    rows, C, ldg = _matrix("grad", grad)
-    if rows != T or C == 0:
-        raise ValueError(f"grad must have {T} rows and at least one column")
-    if weights is None:
-        raise ValueError("combine_rows_backward needs the weights")
-    dt, wdt = dtype_code(grad.dtype), _weights(weights, position)
-    ldy = C
-    if y is not None:
-        yr, yc, ldy = _matrix("y", y)
-        if yr != T * k or yc != C or y.dtype != grad.dtype:
-            raise ValueError(f"y must be {grad.dtype} of shape ({T * k}, {C})")
-    gy = grad.new_empty((T * k, C)) if need_y else None
-    gw = torch.empty_like(weights) if need_weights else None
-    _call_on(idx, "g2q_combine_rows_backward", _ptr(gy), C, _ptr(gw), grad.data_ptr(), ldg,
-             _ptr(y), ldy, dt, position.data_ptr(), weights.data_ptr(), wdt, T, k, C)
-    return gy, gw
+    return _lib.binding().combine_rows_backward(grad, y, position, weights, need_y, need_weights)

@@ -297,6 +297,29 @@ def test_gradients_that_are_not_needed():
 
 
 @gpu
+def test_second_derivatives_are_refused():
+    g = gen(4)
+    r = moe_utils.route(torch.randint(0, 4, (9, 2), generator=g, device=DEV), 4)
+    x = torch.randn(9, 8, generator=g, device=DEV).requires_grad_()
+    w = torch.rand(9, 2, generator=g, device=DEV).requires_grad_()
+    out = moe_utils.combine(moe_utils.dispatch(x, r), r, w)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out.sum(), x, create_graph=True)
+
+
+@gpu
+def test_rows_changed_in_place_are_noticed():
+    g = gen(4)
+    r = moe_utils.route(torch.randint(0, 4, (9, 2), generator=g, device=DEV), 4)
+    y = torch.randn(18, 8, generator=g, device=DEV)
+    w = torch.rand(9, 2, generator=g, device=DEV).requires_grad_()
+    out = moe_utils.combine(y, r, w)
+    y.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+@gpu
 def test_rows_beyond_32_bit_offsets():
     g = gen(5)
     T, k, C = 40000, 8, 8192  # 2.6e9 elements
