@@ -22,13 +22,12 @@ using rows::of_f;
 
 // G threads per row, UNITS units of 16 elements per thread kept in registers
 // between the maximum and the codes (one read of x).  What is left of a row --
-// the units beyond UNITS * G, a part of a unit at its end, all of a row that is
-// not 16-byte aligned -- goes element by element and is read a second time.
-template <typename S, int G, int UNITS>
+// the units beyond UNITS * G, a part of a unit at its end -- goes element by
+// element and is read a second time.  VEC: rows on 16-byte boundaries.
+template <typename S, int G, int UNITS, bool VEC>
 __global__ void __launch_bounds__(G > 128 ? G : 128)
     quantize_kernel(int8_t* __restrict__ codes, long long ldq, float* __restrict__ scale_out,
-                    const S* __restrict__ x, long long ldx, long long T, int C, bool xvec,
-                    bool qvec) {
+                    const S* __restrict__ x, long long ldx, long long T, int C, bool qvec) {
   constexpr int BLOCK = G > 128 ? G : 128;
   constexpr int PER = BLOCK / G;  // rows per block
   tc::launch_dependents();  // a product that overlaps waits for this kernel to end
@@ -36,14 +35,17 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
   const long long t = blockIdx.x * (long long)PER + threadIdx.x / G;
   const bool live = t < T;
   const S* row = x + (live ? t : 0) * ldx;
-  int whole = xvec && live ? C / 16 : 0;  // units that the unrolled loops take
+  int whole = live ? C / 16 : 0;  // units that the unrolled loops take
   whole = whole < UNITS * G ? whole : UNITS * G;
   const int units = live ? (C + 15) / 16 : 0;
 
   Unit<S> u[UNITS];
 #pragma unroll
   for (int k = 0; k < UNITS; ++k)
-    if (tid + k * G < whole) u[k].load(row + 16 * (tid + k * G));
+    if (tid + k * G < whole) {
+      if (VEC) u[k].load(row + 16 * (tid + k * G));
+      else u[k].load_any(row + 16 * (tid + k * G));
+    }
   unsigned top = 0;
 #pragma unroll
   for (int k = 0; k < UNITS; ++k)
@@ -54,7 +56,11 @@ __global__ void __launch_bounds__(G > 128 ? G : 128)
     v.load_part(row + 16LL * i, C - 16 * i);
     top = max(top, top_of<S>(v.top_bits()));
   }
-  top = __reduce_max_sync(0xffffffffu, top);
+  if constexpr (G < 32) {  // the lanes of this row
+    top = __reduce_max_sync(((1u << G) - 1u) << ((threadIdx.x & 31) / G * G), top);
+  } else {
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
   if constexpr (G > 32) {
     __shared__ unsigned warp_top[BLOCK / 32];
     if ((threadIdx.x & 31) == 0) warp_top[threadIdx.x >> 5] = top;
@@ -87,8 +93,12 @@ static int launch_quantize(int8_t* codes, long long ldq, float* scale, const S* 
   if (blocks > 0x7fffffffLL || C > 0x7fffff00LL) return G2Q_ERR_UNSUPPORTED;
   const bool xvec = rows::aligned(x, 16) && (T <= 1 || (ldx * (long long)sizeof(S)) % 16 == 0);
   const bool qvec = rows::aligned(codes, 16) && (T <= 1 || ldq % 16 == 0);
-  quantize_kernel<S, G, UNITS><<<(unsigned)blocks, BLOCK, 0, st>>>(codes, ldq, scale, x, ldx, T,
-                                                                   (int)C, xvec, qvec);
+  if (xvec)
+    quantize_kernel<S, G, UNITS, true><<<(unsigned)blocks, BLOCK, 0, st>>>(codes, ldq, scale, x,
+                                                                           ldx, T, (int)C, qvec);
+  else
+    quantize_kernel<S, G, UNITS, false><<<(unsigned)blocks, BLOCK, 0, st>>>(codes, ldq, scale, x,
+                                                                            ldx, T, (int)C, qvec);
   G2Q_CHECK_LAUNCH();
   return G2Q_OK;
 }
@@ -99,10 +109,11 @@ static int quantize_rows(int8_t* codes, long long ldq, float* scale, const void*
   const S* xs = static_cast<const S*>(x);
   // Few rows: sixteen warps each, so that more SMs and more loads are at work.
   if (T < 2 * 148) return launch_quantize<S, 512, 2>(codes, ldq, scale, xs, ldx, T, C, st);
-  // Else as few warps per row as its elements in registers allow (128 or 64 bytes
-  // of them per thread): the row's reduction and division serve the most elements.
+  // Else as few lanes per row as its elements in registers allow (128 bytes of them
+  // per thread): the row's reduction and division serve the most elements.
   constexpr int U = sizeof(S) == 2 ? 4 : 2;
-  if (C <= 1024) return launch_quantize<S, 32, 2>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C <= 256 * U) return launch_quantize<S, 16, U>(codes, ldq, scale, xs, ldx, T, C, st);
+  if (C <= 512 * U) return launch_quantize<S, 32, U>(codes, ldq, scale, xs, ldx, T, C, st);
   if (C <= 1024 * U) return launch_quantize<S, 64, U>(codes, ldq, scale, xs, ldx, T, C, st);
   if (C <= 2048 * U) return launch_quantize<S, 128, U>(codes, ldq, scale, xs, ldx, T, C, st);
   if (C <= 4096 * U) return launch_quantize<S, 256, U>(codes, ldq, scale, xs, ldx, T, C, st);

@@ -30,6 +30,18 @@ struct Unit {
       raw[4 * i + 3] = v.w;
     }
   }
+  // the same from any address
+  __device__ __forceinline__ void load_any(const S* p) {
+    if (sizeof(S) == 4 || (reinterpret_cast<uintptr_t>(p) & 3) == 0) {
+#pragma unroll
+      for (int i = 0; i < W; ++i) raw[i] = __ldg(reinterpret_cast<const uint32_t*>(p) + i);
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+      for (int i = 0; i < W; ++i)
+        raw[i] = (uint32_t)__ldg(h + 2 * i) | (uint32_t)__ldg(h + 2 * i + 1) << 16;
+    }
+  }
   __device__ __forceinline__ void load_part(const S* p, int have) {
     S e[16];
 #pragma unroll
