@@ -232,7 +232,8 @@ def test_quantize_strides(dtype, pad, first):
 
 SHAPES = [(1, 1, 1), (1, 64, 16), (1, 1000, 4096), (7, 130, 100), (16, 257, 144), (17, 96, 512),
           (33, 520, 1040), (64, 128, 128), (100, 256, 2048), (129, 300, 272), (255, 256, 256),
-          (256, 512, 384), (257, 1376, 512), (700, 1000, 1008), (1, 8, 20000)]
+          (256, 512, 384), (257, 1376, 512), (700, 1000, 1008), (1, 8, 20000), (1, 8000, 1040),
+          (8, 100, 1024), (5, 9000, 500), (12, 70, 1000), (16, 48, 4112), (2, 40, 5000)]
 
 
 @gpu
