@@ -40,6 +40,8 @@ constexpr int STAGE_BYTES = KC * 2 * OP_BYTES;
 constexpr int STAGES = 3;
 constexpr int EPI_WARPS = 8;
 constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int PARTS = EPI_WARPS / 4;        // warps per quadrant, taking turns at blocks of 32 tokens
+constexpr int WARP_TOK = TOK / PARTS;       // tokens per warp and tile
 constexpr int STRIP_BYTES = 16 * 32 * 2;  // 16 tokens x 32 channels of 2 bytes
 constexpr int RASTER = 8;            // row pieces walked together (4 and 16 measured the same)
 constexpr int BAR_BYTES = 256;       // barriers, TMEM address, abort flag
@@ -258,9 +260,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   uint8_t* strips = smem + STAGES * STAGE_BYTES + BAR_BYTES;  // [EPI_WARPS][STRIP_BYTES]
-  float* sa_s = reinterpret_cast<float*>(strips + EPI_WARPS * STRIP_BYTES);  // [2][TOK]
+  float* sa_s = reinterpret_cast<float*>(strips + EPI_WARPS * STRIP_BYTES);  // [EPI_WARPS][2][WARP_TOK]
   Table table;
-  table.first = reinterpret_cast<int32_t*>(sa_s + 2 * TOK);
+  table.first = reinterpret_cast<int32_t*>(sa_s + EPI_WARPS * 2 * WARP_TOK);
   table.lo = table.first + p.groups + 2;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else {
     // warp w reads TMEM lanes 32 (w % 4) .. + 31 (channels) of this CTA; the
     // warps of a quadrant take turns at blocks of 32 tokens
-    const int q = warp & 3, part = (warp - 2) / 4, et = threadIdx.x - 64;
+    const int q = warp & 3, part = (warp - 2) / 4;
     const uint32_t acce_lead = mapa_shared(acce0, 0);
     S* out = static_cast<S*>(p.out);
     // 16-bit outputs leave as 16-byte pieces of token rows, through a strip of 16
@@ -425,14 +427,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t st_row = smem_u32(strip) + (lane % 8) * 64 + (((lane / 8) ^ (lane % 8 / 2)) * 16);
     const uint8_t* ld_row = strip + (lane / 4) * 64 + (((lane % 4) ^ (lane / 4 / 2 % 4)) * 16);
     Tile t, next;
-    float sa_next = 0.f;
+    float* sa_w = sa_s + (warp - 2) * 2 * WARP_TOK;
+    float sa_next[WARP_TOK / 32];  // lane: one token of each block
     Channels ch_next;
     // a tile's scales are loaded one tile ahead; zeros where there is no such
     // row or channel, and for rows behind the last group
     auto fetch = [&](int w) {
       next = decode(a, table, w);
       const bool zero = next.group == p.groups;
-      sa_next = !zero && et < next.rows ? p.sa[next.row0 + et] : 0.f;
+#pragma unroll
+      for (int b = 0; b < WARP_TOK / 32; ++b) {
+        const int c = 32 * (part + b * PARTS) + lane;
+        sa_next[b] = !zero && c < next.rows ? p.sa[next.row0 + c] : 0.f;
+      }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (u > 0 && !frag) break;
@@ -448,9 +455,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (; w < total; w += step, ++turn) {
       t = next;
       const Channels ch = ch_next;
-      float* sa = sa_s + (turn & 1) * TOK;
-      if (et < TOK) sa[et] = sa_next;
-      asm volatile("bar.sync 1, %0;" ::"n"(32 * EPI_WARPS) : "memory");
+      float* sa = sa_w + (turn & 1) * WARP_TOK;
+#pragma unroll
+      for (int b = 0; b < WARP_TOK / 32; ++b) sa[32 * b + lane] = sa_next[b];
+      __syncwarp();
       if (w + step < total) fetch(w + step);
       const bool zero = t.group == p.groups;
       const int buf = tc & 1;
@@ -464,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const uint32_t base = tmem + (uint32_t)(buf * TOK) + ((uint32_t)(q * 32) << 16);
       const long long n0 = t.ch0 + 128 * (long long)rank + q * 32;
       const long long n = p.N - n0;  // channels of the strip (may be none)
-      for (int c0 = 32 * part; c0 < t.rows; c0 += 8 * EPI_WARPS) {
+      for (int c0 = 32 * part, cw = 0; c0 < t.rows; c0 += 32 * PARTS, cw += 32) {
         const long long row = t.row0 + c0;
         const int rows = t.rows - c0;
         if (frag) {
@@ -484,7 +492,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {  // 8 of them
               const float2 s2 =
-                  *reinterpret_cast<const float2*>(sa + c0 + 16 * h + 8 * j + 2 * (lane % 4));
+                  *reinterpret_cast<const float2*>(sa + cw + 16 * h + 8 * j + 2 * (lane % 4));
               uint32_t m[4];
 #pragma unroll
               for (int u = 0; u < 4; ++u) {
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int c = 0; c < 32; ++c)
               if (c < rows)
-                dst[c * p.ldo] = of_f<S>(scaled((int)r[c], sa[c0 + c], ch.sb[0], ch.bias[0]));
+                dst[c * p.ldo] = of_f<S>(scaled((int)r[c], sa[cw + c], ch.sb[0], ch.bias[0]));
           }
         }
       }
@@ -654,7 +662,7 @@ template <typename S>
 static int launch_tc(const Maps& maps, const TcArgs& a, long long tiles, bool overlap,
                      cudaStream_t st) {
   const int smem = STAGES * STAGE_BYTES + 1024 + BAR_BYTES + EPI_WARPS * STRIP_BYTES +
-                   2 * TOK * (int)sizeof(float) +
+                   EPI_WARPS * 2 * WARP_TOK * (int)sizeof(float) +
                    (int)(2 * a.p.groups + 4) * (int)sizeof(int32_t);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return G2Q_ERR_CUDA;
