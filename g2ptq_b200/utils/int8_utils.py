@@ -13,11 +13,10 @@ from .. import ops
 
 
 def _int8_rows(codes):
-    """``codes`` in memory with rows on 16-byte boundaries."""
+    """``codes`` with rows padded with zeros to 16-byte boundaries."""
     *lead, cols = codes.shape
     out = torch.zeros(*lead, ops.int8_row_stride(cols), dtype=torch.int8, device=codes.device)
-    out = out[..., :cols]
-    out.copy_(codes)
+    out[..., :cols].copy_(codes)
     return out
 
 
@@ -61,14 +60,28 @@ def weight_codes(weight, quantizer):
     return q.to(torch.int8), scale.contiguous()
 
 
-class Int8Linear(torch.nn.Module):
-    """A linear that holds int8 codes and channel scales."""
+class _Int8Weight(torch.nn.Module):
+    """int8 codes and channel scales.  The buffer ``rows`` holds the padded rows (so
+    that moving or copying the module keeps their alignment), ``codes`` is the
+    view of the columns."""
+
+    def __init__(self, codes, scale):
+        super().__init__()
+        self.out_features, self.in_features = codes.shape[-2:]
+        self.register_buffer("rows", _int8_rows(codes))
+        self.register_buffer("scale", scale.detach().float().contiguous())
+
+    @property
+    def codes(self):
+        rows = self.rows
+        return rows if rows.shape[-1] == self.in_features else rows[..., :self.in_features]
+
+
+class Int8Linear(_Int8Weight):
+    """A linear that holds int8 codes ``[N, K]`` and channel scales ``[N]``."""
 
     def __init__(self, codes, scale, bias=None):
-        super().__init__()
-        self.out_features, self.in_features = codes.shape
-        self.register_buffer("codes", _int8_rows(codes))
-        self.register_buffer("scale", scale.detach().reshape(-1).float().contiguous())
+        super().__init__(codes, scale.reshape(-1))
         self.register_buffer("bias", None if bias is None else bias.detach().float().contiguous())
 
     @classmethod
@@ -84,13 +97,9 @@ class Int8Linear(torch.nn.Module):
         return int8_linear(x, self.codes, self.scale, self.bias)
 
 
-class Int8Experts(torch.nn.Module):
-    """The same projection of every expert of an MoE layer, stacked."""
-
-    def __init__(self, codes, scale):
-        super().__init__()
-        self.register_buffer("codes", _int8_rows(codes))
-        self.register_buffer("scale", scale.detach().float().contiguous())
+class Int8Experts(_Int8Weight):
+    """The same projection of every expert of an MoE layer, stacked: codes
+    ``[E, N, K]`` and scales ``[E, N]``."""
 
     @classmethod
     def from_linears(cls, linears, quantizers):

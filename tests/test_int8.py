@@ -7,6 +7,7 @@ once each (2^-24 relative to the scaled sum, or to the result), the output type
 once more (half its spacing)."""
 
 import ctypes
+import os
 
 import pytest
 import torch
@@ -15,6 +16,15 @@ from g2ptq_b200 import _lib, ops
 from g2ptq_b200.utils import int8_utils, moe_utils
 
 gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from g2ptq_b200 import build
+    if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(build.BINDING)):
+        build.build()
+
+
 DEV = "cuda"
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 U = 2.0 ** -24  # half the relative spacing of fp32
@@ -60,8 +70,13 @@ def codes_of(shape, g, lo=-128):
     return torch.randint(lo, 128, shape, generator=g, device=DEV, dtype=torch.int8)
 
 
+def aligned(codes):
+    """The same codes with rows on 16-byte boundaries."""
+    return int8_utils._int8_rows(codes)[..., :codes.shape[-1]]
+
+
 def aligned_codes(shape, g):
-    return int8_utils._int8_rows(codes_of(shape, g))
+    return aligned(codes_of(shape, g))
 
 
 def gen(seed=0):
@@ -290,8 +305,8 @@ def test_int8_matmul_unaligned_rows(M, N, K, pa, pb):
 def test_int8_matmul_extreme_codes(M):
     # the largest sums: every product 128 * 128 or -128 * 127
     K = ops.INT8_MAX_K - 15
-    a = int8_utils._int8_rows(torch.full((M, K), -128, dtype=torch.int8, device=DEV))
-    b = int8_utils._int8_rows(torch.full((3, K), -128, dtype=torch.int8, device=DEV))
+    a = aligned(torch.full((M, K), -128, dtype=torch.int8, device=DEV))
+    b = aligned(torch.full((3, K), -128, dtype=torch.int8, device=DEV))
     b[1] = 127
     sa, sb = torch.ones(M, device=DEV), torch.ones(3, device=DEV)
     check_product(ops.int8_matmul(a, sa, b, sb, out_dtype=torch.float32), a, sa, b, sb, None)
@@ -487,6 +502,27 @@ def test_linear_from_a_quantized_weight():
     assert bool(((back - w).abs() <= U * w.abs() + 1e-30).all())
     q, s = plain_quantize(x.reshape(-1, 256))
     check_product(m(x).reshape(-1, 192), q, s, m.codes, m.scale, lin.bias.data)
+
+
+@gpu
+@pytest.mark.parametrize("K", [96, 100])
+def test_modules_keep_their_layout(K):
+    """Copies, moves and state dicts of a module keep rows that the tensor cores
+    take, and its results."""
+    import copy
+    g = gen(K)
+    m = int8_utils.Int8Linear(codes_of((70, K), g), torch.rand(70, generator=g, device=DEV),
+                              torch.randn(70, generator=g, device=DEV))
+    x = torch.randn(50, K, generator=g, device=DEV)
+    want = m(x)
+    other = int8_utils.Int8Linear(codes_of((70, K), g), torch.rand(70, generator=g, device=DEV),
+                                  torch.zeros(70, device=DEV))
+    other.load_state_dict(m.state_dict())
+    for mod in (copy.deepcopy(m), copy.deepcopy(m).cpu().to(DEV), other):
+        assert mod.codes.shape == (70, K) and mod.codes.stride(0) % 16 == 0
+        assert torch.equal(mod.codes, m.codes) and torch.equal(mod(x), want)
+    e = int8_utils.Int8Experts(codes_of((3, 20, K), g), torch.ones(3, 20, device=DEV))
+    assert e.codes.shape == (3, 20, K) and e.codes.stride(1) % 16 == 0
 
 
 @gpu

@@ -7,6 +7,7 @@ output's type; a dot product over C columns adds at most ceil(C / 32) + 25
 terms in a chain (columns per lane, pieces of at most 16, the tree)."""
 
 import ctypes
+import os
 
 import pytest
 import torch
@@ -15,6 +16,15 @@ from g2ptq_b200 import _lib, ops
 from g2ptq_b200.utils import moe_utils
 
 gpu = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from g2ptq_b200 import build
+    if not (os.path.exists(_lib.LIB_PATH) and os.path.exists(build.BINDING)):
+        build.build()
+
+
 DEV = "cuda"
 DTYPES = [torch.bfloat16, torch.float16, torch.float32]
 U = 2.0 ** -24
