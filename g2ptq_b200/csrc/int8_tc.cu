@@ -21,6 +21,12 @@
 // (leader) MMA issuer, warps 2-9 epilogue.  Every wait is bounded as in the
 // Gram kernels; on expiry G2Q_ERR_TIMEOUT goes to the status word and the CTAs
 // wind down.
+//
+// Measured: 16384 x 14336 x 4096 in 596-615 us (3.2 POP/s, tensor pipe 88.6 %
+// active; 730-770 us once the card is at its power limit), bound by the pipe;
+// 65536 rows of 768 through 128 experts of 2048 channels in 123-129 us, bound by
+// the epilogue (6.2k cycles per tile, of which the MMAs need 3.05k); 24 tokens
+// through 14336 x 4096 in 17 us with the quantization, bound by reading the weight.
 #include "int8.cuh"
 #include "rows.cuh"
 #include "tc_ptx.cuh"
