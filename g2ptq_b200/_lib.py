@@ -156,7 +156,7 @@ def load():
 _BOUND = ("g2q_quantize_tokens", "g2q_int8_matmul", "g2q_int8_matmul_workspace_bytes",
           "g2q_int8_matmul_grouped", "g2q_int8_linear", "g2q_int8_linear_workspace_bytes",
           "g2q_route", "g2q_route_workspace_bytes", "g2q_dispatch_rows", "g2q_combine_rows",
-          "g2q_combine_rows_backward")
+          "g2q_combine_rows_backward", "g2q_status_string")
 _binding = None
 
 

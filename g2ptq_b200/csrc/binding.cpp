@@ -35,7 +35,7 @@ constexpr int64_t kMaxExperts = 1024;
   X(g2q_quantize_tokens) X(g2q_int8_matmul) X(g2q_int8_matmul_workspace_bytes)               \
   X(g2q_int8_matmul_grouped) X(g2q_int8_linear) X(g2q_int8_linear_workspace_bytes)           \
   X(g2q_route) X(g2q_route_workspace_bytes) X(g2q_dispatch_rows) X(g2q_combine_rows)         \
-  X(g2q_combine_rows_backward)
+  X(g2q_combine_rows_backward) X(g2q_status_string)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -58,7 +58,9 @@ void bind(const py::dict& addresses, py::object error, py::object status_word) {
 
 void run(const char* name, int status) {
   if (status >= 0) return;
-  py::gil_scoped_acquire gil;
+  // (a backward runs without the interpreter's lock: a plain error there)
+  TORCH_CHECK(PyGILState_Check(), name, " failed: ", api.g2q_status_string(status), " (status ",
+              status, ")");
   py::object e = (*g_error)(name, status);
   PyErr_SetObject(reinterpret_cast<PyObject*>(Py_TYPE(e.ptr())), e.ptr());
   throw py::error_already_set();

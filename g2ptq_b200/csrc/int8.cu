@@ -130,10 +130,9 @@ int quantize_tokens(int8_t* codes, long long ldq, float* scale, const void* x, i
 }
 
 // ---------------------------------------------------------------------------
-// product on the CUDA cores: operands of any alignment
+// product on the CUDA cores: operands of any alignment (a weight with rows at odd
+// strides; 16384 x 14336 x 4096 took 18.8 ms)
 // ---------------------------------------------------------------------------
-
-// (a user's weight with rows at odd strides; 16384 x 14336 x 4096 took 18.8 ms)
 
 constexpr int ST = 64;   // tile edge (tokens and channels)
 constexpr int SKW = 16;  // 32-bit words of K per step

@@ -168,6 +168,15 @@ def test_refusals():
         ops.int8_matmul_grouped(i8(2, 4), f(2), i8(1, 5, 4).expand(2, 5, 4), f(2, 5), off)
 
 
+@gpu
+def test_library_errors_reach_the_caller():
+    # more row tiles of unaligned operands than a grid has: refused before any launch
+    a = torch.zeros(65536 * 64, 3, dtype=torch.int8, device=DEV)
+    with pytest.raises(_lib.G2QError, match="unsupported"):
+        ops.int8_matmul(a, torch.ones(a.shape[0], device=DEV),
+                        torch.zeros(2, 3, dtype=torch.int8, device=DEV), torch.ones(2, device=DEV))
+
+
 # -- quantization -------------------------------------------------------------
 
 @gpu

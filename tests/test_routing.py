@@ -306,6 +306,28 @@ def test_gradients_that_are_not_needed():
         assert moe_utils.dispatch(go.requires_grad_(), r).grad_fn is None
 
 
+def test_library_errors_keep_their_type():
+    """A negative status of the library is a G2QError through the native binding too."""
+    p = torch.zeros(2, 2, dtype=torch.int32)
+    mod = _lib.binding()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        mod.combine_rows(torch.zeros(4, 4), p, None)
+    assert issubclass(_lib.G2QError, RuntimeError)
+
+
+@gpu
+def test_a_refused_size_is_a_library_error():
+    # more elements per slot than the library indexes: refused before any launch
+    lib = _lib.load()
+    x = torch.zeros(2, 8, device=DEV)
+    pos = torch.zeros(2, 2, dtype=torch.int32, device=DEV)
+    assert lib.g2q_dispatch_rows(x.data_ptr(), 4, x.data_ptr(), 8, 4, pos.data_ptr(), 2, 2, 8,
+                                 None) == _lib.G2Q_ERR_INVALID_ARG
+    with pytest.raises(_lib.G2QError, match="invalid argument"):
+        _lib.call("g2q_dispatch_rows", x.data_ptr(), 4, x.data_ptr(), 8, 4, pos.data_ptr(), 2, 2,
+                  8, None)
+
+
 @gpu
 def test_second_derivatives_are_refused():
     g = gen(4)
