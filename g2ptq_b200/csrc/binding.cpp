@@ -240,8 +240,9 @@ Tensor linear(const On& on, const Tensor& x, const Matrix& m, const Tensor& code
   const int dt = dtype_code(x.scalar_type());
   Tensor out = at::empty({m.rows, w.N}, x.options());
   const int8_t* b = bdata(codes);
-  const int aligned =
-      ((reinterpret_cast<uintptr_t>(b) | (uintptr_t)w.ldb | (uintptr_t)w.gs) & 15) == 0;
+  // strides that are never stepped over do not count
+  const int64_t ldb = w.N > 1 ? w.ldb : 0, gs = w.E > 1 ? w.gs : 0;
+  const int aligned = ((reinterpret_cast<uintptr_t>(b) | (uintptr_t)ldb | (uintptr_t)gs) & 15) == 0;
   Bytes ws(api.g2q_int8_linear_workspace_bytes(m.rows, w.N, m.cols, w.E, aligned), x);
   G2Q_RUN(g2q_int8_linear, out.data_ptr(), dt, w.N, x.const_data_ptr(), dt, m.ld, b, w.ldb, w.gs,
           fdata(scale), bias, offsets, w.E, m.rows, w.N, m.cols, ws.get(), ws.n,

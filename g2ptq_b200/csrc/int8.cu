@@ -310,7 +310,6 @@ extern "C" size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t 
       N > i8::kMaxRows || G > i8::kMaxGroups)
     return 0;
   i8::Product p = {};
-  p.b = reinterpret_cast<const int8_t*>(aligned ? 256 : 257);
   p.lda = p.ldb = (K + 15) / 16 * 16;
   p.b_gs = p.ldb * N;
   p.groups = G > 0 ? G : 1;
@@ -318,7 +317,16 @@ extern "C" size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t 
   p.M = M;
   p.N = N;
   p.K = K;
-  return i8::linear_workspace(p);
+  p.b = reinterpret_cast<const int8_t*>(aligned ? 256 : 257);
+  size_t need = i8::linear_workspace(p);
+  // the tensor-core product ignores the row stride of a single channel and the stride
+  // of a single expert: with `aligned` 0 because of such a stride it still runs
+  if (!aligned && (N == 1 || G == 1)) {
+    p.b = reinterpret_cast<const int8_t*>(256);
+    const size_t other = i8::linear_workspace(p);
+    need = other > need ? other : need;
+  }
+  return need;
 }
 
 extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void* x, int x_dtype,

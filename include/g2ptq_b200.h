@@ -491,7 +491,9 @@ int g2q_int8_matmul_grouped(void* out, int out_dtype, int64_t ldo, const int8_t*
  * (G = 0, offsets NULL) or g2q_int8_matmul_grouped (G > 0, bias NULL) in one
  * call, the product starting while the quantization ends.  `workspace`: 16-byte
  * aligned, g2q_int8_linear_workspace_bytes(M, N, K, G, aligned) bytes (may be 0),
- * with aligned != 0 only where b's base and strides are multiples of 16 bytes. */
+ * with aligned != 0 only where b's base, its row stride (of more than one
+ * channel) and its group stride (of more than one group) are multiples of 16
+ * bytes. */
 size_t g2q_int8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K, int64_t G, int aligned);
 int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void* x, int x_dtype, int64_t ldx,
                     const int8_t* b, int64_t ldb, int64_t b_gs, const float* b_scale,

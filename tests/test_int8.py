@@ -131,6 +131,20 @@ def test_quantizer_kinds_are_refused():
         int8_utils.weight_codes(torch.zeros(2, 4), q)
 
 
+@pytest.mark.parametrize("M,K", [(17, 4100), (64, 4100), (200, 2050), (1000, 4100), (200, 4090),
+                                 (4096, 8200)])
+@pytest.mark.parametrize("G", [0, 1])
+def test_one_channel_workspace(M, K, G):
+    """The stride of a single channel does not decide whether its rows are aligned, so
+    neither answer may leave out what the product's ranges of K need."""
+    lib = _lib.load()
+    codes = -(-M * ops.int8_row_stride(K) // 256) * 256 + -(-4 * M // 256) * 256
+    product = lib.g2q_int8_matmul_workspace_bytes(M, 1, K) if G == 0 else 0
+    assert G == 1 or K < 4000 or product > 0
+    for aligned in (0, 1):
+        assert lib.g2q_int8_linear_workspace_bytes(M, 1, K, G, aligned) >= codes + product
+
+
 # -- GPU: refusals ------------------------------------------------------------
 
 @gpu
@@ -459,6 +473,27 @@ def test_int8_linear_is_its_two_steps(M, N, K):
         got = int8_utils.int8_linear(x, b, sb)
     assert torch.equal(got, want)
     assert torch.equal(ops.int8_linear(x, b.contiguous(), sb), want)  # rows of any alignment
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K", [(1, 4100), (5, 4100), (17, 4100), (64, 1666), (64, 4100),
+                                 (200, 2050), (200, 4096), (1000, 4100), (4096, 8200)])
+def test_int8_linear_one_channel(dtype, M, K):
+    """One output channel, its row's stride anything: K itself, or what a view has."""
+    g = gen(M + K)
+    x = torch.randn(M, K, generator=g, device=DEV).to(dtype)
+    codes, scale = codes_of((1, K), g), torch.rand(1, generator=g, device=DEV)
+    bias = torch.randn(1, generator=g, device=DEV)
+    q, s = plain_quantize(x)
+    wide = torch.zeros(1, K + 5, dtype=torch.int8, device=DEV)
+    wide[:, :K] = codes
+    for c in (codes, aligned(codes), wide[:, :K]):
+        check_product(int8_utils.int8_linear(x, c, scale, bias), q, s, codes, scale, bias)
+    check_product(int8_utils.Int8Linear(codes, scale)(x), q, s, codes, scale, None)
+    off = torch.tensor([0, M], dtype=torch.int32, device=DEV)
+    check_product(int8_utils.int8_experts(x, codes[None], scale[None], off), q, s, codes, scale,
+                  None)
 
 
 @gpu
