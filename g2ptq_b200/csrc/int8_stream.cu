@@ -39,11 +39,14 @@ __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, ui
 
 // Bytes k .. k + 15 of a row of K bytes, missing ones zero.  ONCE: read a single
 // time (the weight), so not kept (23.5 -> 20.8 us for four tokens' 128 experts).
+// Else the tokens' codes: the kernel before this one may write them while this grid
+// is already resident, so they are not read-only for its whole life and take an
+// ordinary load, behind wait_predecessor().
 template <bool ONCE>
 __device__ __forceinline__ uint4 load16(const int8_t* row, long long k, long long K) {
   if (k + 16 <= K) {
     const uint4* v = reinterpret_cast<const uint4*>(row + k);
-    return ONCE ? __ldcs(v) : __ldg(v);
+    return ONCE ? __ldcs(v) : *v;
   }
   uint32_t w[4] = {0, 0, 0, 0};
   if (k < K) {

@@ -576,12 +576,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// Adds the K ranges' sums and scales them.
+// Adds the K ranges' sums and scales them.  The sums and the tokens' scales are
+// written by kernels that may still run when this grid starts: no read-only loads.
 template <typename S>
 __global__ void __launch_bounds__(256)
-    finish_kernel(S* __restrict__ out, long long ldo, const int32_t* __restrict__ part, int splits,
-                  const float* __restrict__ sa, const float* __restrict__ sb,
-                  const float* __restrict__ bias, long long M, long long N) {
+    finish_kernel(S* __restrict__ out, long long ldo, const int32_t* part, int splits,
+                  const float* sa, const float* __restrict__ sb, const float* __restrict__ bias,
+                  long long M, long long N) {
   wait_predecessor();
   for (long long m = blockIdx.y; m < M; m += gridDim.y) {
     const float s = sa[m];

@@ -476,6 +476,42 @@ def test_int8_linear_is_its_two_steps(M, N, K):
 
 
 @gpu
+@pytest.mark.parametrize("M,N,K", [(8, 4096, 4096), (3, 300, 20000), (16, 512, 2064), (64, 520, 1040),
+                                   (200, 512, 14336), (700, 1000, 1008)])
+def test_int8_linear_of_changing_inputs(M, N, K):
+    """Back to back calls whose inputs differ and whose workspace is the same memory:
+    every product reads its own call's codes and scales, not what the call before
+    left there while the quantization was still writing."""
+    g = gen(M + N)
+    b, sb = aligned_codes((N, K), g), torch.rand(N, generator=g, device=DEV)
+    xs = [torch.randn(M, K, generator=g, device=DEV) * 2.0 ** (i % 5) for i in range(12)]
+    pairs = [ops.quantize_tokens(x) for x in xs]
+    want = [ops.int8_matmul(q, s, b, sb, out_dtype=torch.float32) for q, s in pairs]
+    torch.cuda.synchronize()
+    got = [int8_utils.int8_linear(x, b, sb) for x in xs]
+    for a, w in zip(got, want):
+        assert torch.equal(a, w)
+
+
+@gpu
+@pytest.mark.parametrize("R,E", [(32, 128), (900, 4)])
+def test_int8_experts_of_changing_inputs(R, E):
+    g = gen(R)
+    N, K = 200, 2048
+    b, sb = aligned_codes((E, N, K), g), torch.rand(E, N, generator=g, device=DEV)
+    off = torch.zeros(E + 1, dtype=torch.int32, device=DEV)
+    off[1:] = torch.bincount(torch.randint(0, E, (R - 3,), generator=g, device=DEV),
+                             minlength=E).cumsum(0)  # three rows without an expert
+    xs = [torch.randn(R, K, generator=g, device=DEV) * 2.0 ** (i % 5) for i in range(12)]
+    pairs = [ops.quantize_tokens(x) for x in xs]
+    want = [ops.int8_matmul_grouped(q, s, b, sb, off, out_dtype=torch.float32) for q, s in pairs]
+    torch.cuda.synchronize()
+    got = [int8_utils.int8_experts(x, b, sb, off) for x in xs]
+    for a, w in zip(got, want):
+        assert torch.equal(a, w) and not bool(a[-3:].any())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,K", [(1, 4100), (5, 4100), (17, 4100), (64, 1666), (64, 4100),
                                  (200, 2050), (200, 4096), (1000, 4100), (4096, 8200)])
