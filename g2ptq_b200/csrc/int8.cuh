@@ -43,16 +43,6 @@ static inline long long range_slots(const Product& p, int tile) {
   return p.offsets ? full + (p.groups < p.M ? p.groups : p.M) : full;
 }
 
-// Rows of group g alone (group == groups: the rows behind the last one), in
-// bounds whatever the offsets hold.
-__device__ __forceinline__ void group_bounds(const Product& p, long long g, long long* lo,
-                                             long long* hi) {
-  long long a = g == 0 ? 0 : p.offsets[g], b = g < p.groups ? (long long)p.offsets[g + 1] : p.M;
-  a = a < 0 ? 0 : (a > p.M ? p.M : a);
-  *lo = a;
-  *hi = b < a ? a : (b > p.M ? p.M : b);
-}
-
 // First row of group g (of group == groups: of the rows behind the last one;
 // beyond: M), for 32 neighbouring g of a warp's lanes in ascending calls with
 // *top = 0 before the first: the running maximum of the offsets within [0, M],

@@ -58,17 +58,37 @@ __device__ __forceinline__ uint4 load16(const int8_t* row, long long k, long lon
 }
 
 // The slot-th group that has rows (counting the rows behind the last group as
-// one more); false where there are fewer.  By each warp alone.
+// one more); false where there are fewer.  By each warp alone.  Groups as
+// group_start has them: while the offsets ascend within [0, M] that is what stands
+// there; from the first that does not, every warp that needs it takes the way of the
+// running maximum.
 __device__ __forceinline__ bool find_group(const Product& p, int slot, int* group, long long* lo,
                                            long long* hi) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, wanted = slot;
   for (int g0 = 0; g0 <= p.groups; g0 += 128) {
-    long long from[4], to[4];
+    int from[4], to[4];
+    bool ascend = true;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const int g = g0 + 32 * i + lane;
       from[i] = to[i] = 0;
-      if (g0 + 32 * i + lane <= p.groups)
-        group_bounds(p, g0 + 32 * i + lane, &from[i], &to[i]);
+      if (g <= p.groups) {
+        from[i] = g == 0 ? 0 : p.offsets[g];
+        to[i] = g < p.groups ? p.offsets[g + 1] : (int)p.M;
+        ascend = ascend && from[i] <= to[i] && to[i] <= p.M;
+      }
+    }
+    if (!__all_sync(0xffffffffu, ascend)) {
+      // pieces of M rows: one to a group
+      Range r = {0, -1, 0};
+      find_range(p, wanted, (int)p.M, &r);
+      const int src = __ffs(__ballot_sync(0xffffffffu, r.rows >= 0)) - 1;
+      const long long row0 = __shfl_sync(0xffffffffu, r.row0, src);
+      const int rows = __shfl_sync(0xffffffffu, r.rows, src);
+      *group = __shfl_sync(0xffffffffu, r.group, src);
+      *lo = row0;
+      *hi = row0 + rows;
+      return rows > 0;
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {

@@ -410,6 +410,53 @@ def test_grouped_offsets_stay_in_bounds(bad):
         check_product(got[30:], a[30:], sa[30:], b[2], sb[2], None)
 
 
+def partition(off, M):
+    """The rows of each group, and behind the last, as the running maximum of the
+    offsets within [0, M] cuts them."""
+    cut, top = [0], 0
+    for v in off[1:]:
+        top = max(top, min(v, M))
+        cut.append(top)
+    return cut + [M]
+
+
+BAD_OFFSETS = {
+    "descending": lambda o, n: o[:n // 2] + [o[n // 2] // 3] + o[n // 2 + 1:],
+    "saw": lambda o, n: [v if i % 2 else v // 2 for i, v in enumerate(o)],
+    "negative": lambda o, n: o[:n // 3] + [-5] + o[n // 3 + 1:],
+    "first": lambda o, n: [o[n // 2]] + o[1:],
+    "beyond": lambda o, n: o[:-1] + [o[-1] + 1000],
+    "all beyond": lambda o, n: [0] + [2 ** 31 - 1] * (len(o) - 1),
+    "all negative": lambda o, n: [-2 ** 31] * len(o),
+    "falling": lambda o, n: o[::-1],
+}
+
+
+@gpu
+@pytest.mark.parametrize("bad", sorted(BAD_OFFSETS))
+# few rows per group (the streaming kernel), many, and rows off 16-byte boundaries
+@pytest.mark.parametrize("R,E,K", [(60, 40, 64), (500, 300, 64), (60, 3, 64), (700, 3, 64),
+                                   (60, 40, 50), (3, 2, 64)])
+def test_any_offsets_partition_the_rows(bad, R, E, K):
+    g = gen(R + E)
+    ids = torch.randint(0, E, (R - 2,), generator=g, device=DEV)
+    good = [0] + torch.bincount(ids, minlength=E).cumsum(0).tolist()
+    off = BAD_OFFSETS[bad](good, E)
+    a, b = codes_of((R, K), g), codes_of((E, 24, K), g)
+    a, b = (aligned(a), aligned(b)) if K % 16 == 0 else (a, b)
+    sa, sb = torch.rand(R, generator=g, device=DEV), torch.rand(E, 24, generator=g, device=DEV)
+    poison = torch.full((R, 24), float("nan"), device=DEV)  # what an unwritten row would show
+    del poison
+    got = ops.int8_matmul_grouped(a, sa, b, sb, torch.tensor(off, dtype=torch.int32, device=DEV),
+                                  out_dtype=torch.float32)
+    cut = partition(off, R)
+    for e in range(E):
+        lo, hi = cut[e], cut[e + 1]
+        if hi > lo:
+            check_product(got[lo:hi], a[lo:hi], sa[lo:hi], b[e], sb[e], None)
+    assert not bool((got[cut[E]:] != 0).any())
+
+
 @gpu
 def test_grouped_strided_experts():
     g = gen(9)
