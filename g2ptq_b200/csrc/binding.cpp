@@ -132,6 +132,17 @@ const float* fdata(const optional<Tensor>& t) { return t.has_value() ? fdata(*t)
 const int8_t* bdata(const Tensor& t) { return static_cast<const int8_t*>(t.const_data_ptr()); }
 const int32_t* idata(const Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 
+// An operator that records nothing refuses inputs whose gradient the caller expects,
+// instead of dropping it without a word.
+void no_gradient(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs) {
+    if (!t || !t->defined()) continue;
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), what,
+                " records no gradient: detach its inputs or call it under torch.no_grad()");
+    TORCH_CHECK(!t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+  }
+}
+
 struct Bytes {  // scratch of a call, from the caching allocator
   Tensor t;
   size_t n;
@@ -206,6 +217,7 @@ std::tuple<Tensor, Tensor> quantize_tokens(const Tensor& x) {
 
 Tensor int8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, const Tensor& b_scale,
                    const optional<Tensor>& bias, const py::object& out_dtype) {
+  no_gradient("int8_matmul", {&a_scale, &b_scale, given(bias)});
   On on(a, {&a_scale, &b, &b_scale, given(bias)});
   const Matrix m = codes_of(a, a_scale);
   const Weight w = weight(b, b_scale, m.cols);
@@ -223,6 +235,7 @@ Tensor int8_matmul(const Tensor& a, const Tensor& a_scale, const Tensor& b, cons
 Tensor int8_matmul_grouped(const Tensor& a, const Tensor& a_scale, const Tensor& b,
                            const Tensor& b_scale, const Tensor& offsets,
                            const py::object& out_dtype) {
+  no_gradient("int8_matmul_grouped", {&a_scale, &b_scale});
   On on(a, {&a_scale, &b, &b_scale, &offsets});
   const Matrix m = codes_of(a, a_scale);
   const Weight w = expert_weight(b, b_scale, offsets, m.cols);
@@ -252,6 +265,7 @@ Tensor linear(const On& on, const Tensor& x, const Matrix& m, const Tensor& code
 
 Tensor int8_linear(const Tensor& x, const Tensor& codes, const Tensor& scale,
                    const optional<Tensor>& bias) {
+  no_gradient("int8_linear", {&x, &scale, given(bias)});
   On on(x, {&codes, &scale, given(bias)});
   const Matrix m = matrix("x", x);
   const Weight w = weight(codes, scale, m.cols);
@@ -261,6 +275,7 @@ Tensor int8_linear(const Tensor& x, const Tensor& codes, const Tensor& scale,
 
 Tensor int8_linear_grouped(const Tensor& x, const Tensor& codes, const Tensor& scale,
                            const Tensor& offsets) {
+  no_gradient("int8_linear_grouped", {&x, &scale});
   On on(x, {&codes, &scale, &offsets});
   const Matrix m = matrix("x", x);
   const Weight w = expert_weight(codes, scale, offsets, m.cols);

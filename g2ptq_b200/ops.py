@@ -570,14 +570,16 @@ def quantize_tokens(x):
     fp32): ``scale = max |x| / 127``, ``code = round(x / scale)`` with ties to
     even.  A row whose values are all zero has scale 1; one with an infinity or
     a NaN has scale NaN and codes 0.  Returns ``(codes [T, C], scale [T])``, the
-    codes' rows ``int8_row_stride(C)`` apart."""
+    codes' rows ``int8_row_stride(C)`` apart.  No gradient."""
     return _lib.binding().quantize_tokens(x)
 
 
 def int8_matmul(a, a_scale, b, b_scale, bias=None, out_dtype=torch.bfloat16):
     """``out[m, n] = a_scale[m] * b_scale[n] * sum_k a[m, k] b[n, k] + bias[n]``
     for int8 ``a [M, K]`` and ``b [N, K]``, fp32 scales and bias; the sums are
-    exact.  Rows 16 bytes aligned (``int8_row_stride``) run on the tensor cores."""
+    exact.  Rows 16 bytes aligned (``int8_row_stride``) run on the tensor cores.
+    Like the other 8-bit products it records no gradient and refuses inputs that
+    require one under grad mode."""
     return _lib.binding().int8_matmul(a, a_scale, b, b_scale, bias, out_dtype)
 
 

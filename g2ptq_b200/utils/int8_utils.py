@@ -4,7 +4,8 @@ quantized to int8 codes with one scale per channel.
 Activations are quantized per token as they arrive (the reference's per-token
 symmetric ``ActQuantizer``, utils/quant_utils.py:167-338, which only emulates it
 in the model's type); the codes are multiplied as integers and the sums scaled
-per token and per channel.  Inference only: nothing here records gradients.
+per token and per channel.  Inference only: nothing here records gradients, and
+inputs that require one are refused under grad mode (``RuntimeError``).
 """
 
 import torch
@@ -92,7 +93,6 @@ class Int8Linear(_Int8Weight):
         codes, scale = weight_codes(linear.weight.data, quantizer)
         return cls(codes, scale, linear.bias)
 
-    @torch.no_grad()
     def forward(self, x):
         return int8_linear(x, self.codes, self.scale, self.bias)
 
@@ -106,6 +106,5 @@ class Int8Experts(_Int8Weight):
         pairs = [weight_codes(lin.weight.data, q) for lin, q in zip(linears, quantizers)]
         return cls(torch.stack([c for c, _ in pairs]), torch.stack([s for _, s in pairs]))
 
-    @torch.no_grad()
     def forward(self, rows, offsets):
         return int8_experts(rows, self.codes, self.scale, offsets)

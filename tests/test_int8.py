@@ -145,6 +145,38 @@ def test_one_channel_workspace(M, K, G):
         assert lib.g2q_int8_linear_workspace_bytes(M, 1, K, G, aligned) >= codes + product
 
 
+def test_lost_gradients_are_refused():
+    """Nothing records a gradient here: an input that requires one is refused, not
+    detached without a word."""
+    import torch.autograd.forward_ad as fwad
+    i8 = torch.zeros(3, 4, dtype=torch.int8)
+    one, three = torch.ones(2), torch.ones(3)
+    off = torch.tensor([0, 2], dtype=torch.int32)
+    x = torch.ones(2, 4)
+
+    def grad(t):
+        return t.clone().requires_grad_()
+
+    module = int8_utils.Int8Linear(i8, three)
+    experts = int8_utils.Int8Experts(i8[None], three[None])
+    calls = [lambda f: int8_utils.int8_linear(f(x), i8, three),
+             lambda f: int8_utils.int8_linear(f(x[None]), i8, three),
+             lambda f: int8_utils.int8_linear(x, i8, f(three)),
+             lambda f: int8_utils.int8_linear(x, i8, three, f(three)),
+             lambda f: int8_utils.int8_experts(f(x), i8[None], three[None], off),
+             lambda f: int8_utils.int8_experts(x, i8[None], f(three[None]), off),
+             lambda f: module(f(x)), lambda f: experts(f(x), off),
+             lambda f: ops.int8_matmul(i8[:2], f(one), i8, three),
+             lambda f: ops.int8_matmul_grouped(i8[:2], one, i8[None], f(three[None]), off)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call(grad)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call(grad)
+        with fwad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            call(lambda t: fwad.make_dual(t, torch.ones_like(t)))
+
+
 # -- GPU: refusals ------------------------------------------------------------
 
 @gpu
