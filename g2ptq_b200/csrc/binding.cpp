@@ -132,15 +132,19 @@ const float* fdata(const optional<Tensor>& t) { return t.has_value() ? fdata(*t)
 const int8_t* bdata(const Tensor& t) { return static_cast<const int8_t*>(t.const_data_ptr()); }
 const int32_t* idata(const Tensor& t) { return static_cast<const int32_t*>(t.const_data_ptr()); }
 
-// An operator that records nothing refuses inputs whose gradient the caller expects,
-// instead of dropping it without a word.
+// Derivatives that an operator does not have are refused, not dropped without a
+// word: a forward-mode tangent, and where nothing is recorded any gradient.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t || !t->defined() || !t->_fw_grad(0).defined(), what,
+                " has no forward-mode derivative");
+}
+
 void no_gradient(const char* what, std::initializer_list<const Tensor*> inputs) {
-  for (const Tensor* t : inputs) {
-    if (!t || !t->defined()) continue;
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t->requires_grad()), what,
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t || !t->defined() || !at::GradMode::is_enabled() || !t->requires_grad(), what,
                 " records no gradient: detach its inputs or call it under torch.no_grad()");
-    TORCH_CHECK(!t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
-  }
+  no_tangent(what, inputs);
 }
 
 struct Bytes {  // scratch of a call, from the caching allocator
@@ -455,6 +459,7 @@ struct CombineOnes : torch::autograd::Function<CombineOnes> {
 };
 
 Tensor dispatch_grad(const Tensor& x_in, const Tensor& position) {
+  no_tangent("dispatch", {&x_in});
   const Tensor x = plain_rows(x_in);
   if (!(at::GradMode::is_enabled() && x.requires_grad())) return dispatch_rows(x, position);
   On::check(x, {&position});
@@ -463,6 +468,7 @@ Tensor dispatch_grad(const Tensor& x_in, const Tensor& position) {
 }
 
 Tensor combine_grad(const Tensor& y_in, const Tensor& position, const optional<Tensor>& weights) {
+  no_tangent("combine", {&y_in, given(weights)});
   const Tensor y = plain_rows(y_in);
   const Tensor w = weights ? weights->contiguous() : Tensor();
   if (!(at::GradMode::is_enabled() && (y.requires_grad() || (w.defined() && w.requires_grad()))))

@@ -6,8 +6,8 @@ expert on them and adds the weighted results back, so that the expert
 linears' hooks (``add_batch``, the refresh step's caches) see routed tokens
 only.  Here the pairs are sorted by expert once (``route``), the rows are copied
 into that order in one pass (``dispatch``) and brought back weighted in one
-pass (``combine``), both differentiable (once); ``routed_experts_forward`` is
-that forward.
+pass (``combine``), both differentiable (once, backward; forward-mode tangents are
+refused); ``routed_experts_forward`` is that forward.
 """
 
 import collections

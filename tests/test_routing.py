@@ -315,6 +315,24 @@ def test_library_errors_keep_their_type():
     assert issubclass(_lib.G2QError, RuntimeError)
 
 
+def test_forward_mode_is_refused():
+    """A tangent that nothing carries on is refused, with and without a gradient."""
+    import torch.autograd.forward_ad as fwad
+    p = torch.zeros(2, 2, dtype=torch.int32)
+    r = moe_utils.Routing(p.reshape(-1), p, p[0])
+    x, y, w = torch.ones(2, 4), torch.ones(4, 4), torch.ones(2, 2)
+    with fwad.dual_level():
+        dual = lambda t: fwad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: moe_utils.dispatch(dual(x), r), lambda: moe_utils.combine(dual(y), r),
+                     lambda: moe_utils.combine(dual(y), r, w),
+                     lambda: moe_utils.combine(y, r, dual(w)),
+                     lambda: moe_utils.dispatch(dual(x.clone().requires_grad_()), r)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
 @gpu
 def test_a_refused_size_is_a_library_error():
     # more elements per slot than the library indexes: refused before any launch
