@@ -64,13 +64,24 @@ def weight_codes(weight, quantizer):
 class _Int8Weight(torch.nn.Module):
     """int8 codes and channel scales.  The buffer ``rows`` holds the padded rows (so
     that moving or copying the module keeps their alignment), ``codes`` is the
-    view of the columns."""
+    view of the columns.  Converting the module (``model.to(torch.bfloat16)``,
+    ``.half()``) moves the buffers and leaves their types and values: they are what
+    the quantization chose, whatever type the activations have."""
 
     def __init__(self, codes, scale):
         super().__init__()
         self.out_features, self.in_features = codes.shape[-2:]
         self.register_buffer("rows", _int8_rows(codes))
         self.register_buffer("scale", scale.detach().float().contiguous())
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = dict(self._buffers)
+        super()._apply(fn, *args, **kwargs)
+        for name, old in kept.items():
+            new = self._buffers[name]
+            if old is not None and new.dtype != old.dtype:
+                self._buffers[name] = old.to(new.device)
+        return self
 
     @property
     def codes(self):

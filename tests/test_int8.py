@@ -177,6 +177,32 @@ def test_lost_gradients_are_refused():
             call(lambda t: fwad.make_dual(t, torch.ones_like(t)))
 
 
+CONVERSIONS = [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
+               lambda m: m.float(), lambda m: m.bfloat16().float(), lambda m: m.type(torch.float16)]
+
+
+def converted(make, device):
+    """Each conversion of a model that holds the module, and the module before it."""
+    for convert in CONVERSIONS:
+        mod = make()
+        model = torch.nn.Sequential(torch.nn.Linear(3, 2), mod)
+        before = {k: v.clone() for k, v in mod.state_dict().items()}
+        convert(model.to(device))
+        yield mod, before
+
+
+def test_conversions_keep_codes_and_scales():
+    rows, scale = torch.arange(-50, 50, dtype=torch.int8).reshape(5, 20), torch.rand(5) * 1e-3
+    for make in (lambda: int8_utils.Int8Linear(rows, scale, torch.rand(5)),
+                 lambda: int8_utils.Int8Linear(rows, scale),
+                 lambda: int8_utils.Int8Experts(rows[None], scale[None])):
+        for mod, before in converted(make, "cpu"):
+            after = mod.state_dict()
+            assert sorted(after) == sorted(before)
+            for name, value in before.items():
+                assert after[name].dtype == value.dtype and torch.equal(after[name], value)
+
+
 # -- GPU: refusals ------------------------------------------------------------
 
 @gpu
@@ -682,6 +708,22 @@ def test_modules_keep_their_layout(K):
         assert torch.equal(mod.codes, m.codes) and torch.equal(mod(x), want)
     e = int8_utils.Int8Experts(codes_of((3, 20, K), g), torch.ones(3, 20, device=DEV))
     assert e.codes.shape == (3, 20, K) and e.codes.stride(1) % 16 == 0
+
+
+@gpu
+def test_converted_modules_give_the_same():
+    g = gen(3)
+    codes, scale = codes_of((70, 100), g), torch.rand(70, generator=g, device=DEV) * 1e-2
+    bias = torch.randn(70, generator=g, device=DEV)
+    x = torch.randn(50, 100, generator=g, device=DEV).to(torch.bfloat16)
+    off = torch.tensor([0, 50], dtype=torch.int32, device=DEV)
+    want = int8_utils.Int8Linear(codes, scale, bias)(x)
+    for mod, _ in converted(lambda: int8_utils.Int8Linear(codes.cpu(), scale.cpu(), bias.cpu()), DEV):
+        assert torch.equal(mod(x), want) and mod.codes.stride(0) % 16 == 0
+    want = int8_utils.Int8Experts(codes[None], scale[None])(x, off)
+    for mod, _ in converted(lambda: int8_utils.Int8Experts(codes[None].cpu(), scale[None].cpu()),
+                            DEV):
+        assert torch.equal(mod(x, off), want)
 
 
 @gpu
