@@ -114,7 +114,12 @@ class Int8Experts(_Int8Weight):
 
     @classmethod
     def from_linears(cls, linears, quantizers):
-        pairs = [weight_codes(lin.weight.data, q) for lin, q in zip(linears, quantizers)]
+        """One quantizer per linear.  Linears with a bias are refused: the grouped
+        product has none."""
+        if any(lin.bias is not None for lin in linears):
+            raise ValueError("8-bit experts have no bias; a linear that has one needs Int8Linear")
+        pairs = [weight_codes(lin.weight.data, q)
+                 for lin, q in zip(linears, quantizers, strict=True)]
         return cls(torch.stack([c for c, _ in pairs]), torch.stack([s for _, s in pairs]))
 
     def forward(self, rows, offsets):

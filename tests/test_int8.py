@@ -177,6 +177,19 @@ def test_lost_gradients_are_refused():
             call(lambda t: fwad.make_dual(t, torch.ones_like(t)))
 
 
+def test_experts_from_what_they_cannot_hold(monkeypatch):
+    """A bias, or a linear without its quantizer, is refused instead of left out."""
+    monkeypatch.setattr(int8_utils, "weight_codes",
+                        lambda w, q: (torch.zeros(w.shape, dtype=torch.int8), torch.ones(len(w))))
+    plain = [torch.nn.Linear(8, 4, bias=False) for _ in range(3)]
+    assert int8_utils.Int8Experts.from_linears(plain, [None] * 3).codes.shape == (3, 4, 8)
+    with pytest.raises(ValueError, match="bias"):
+        int8_utils.Int8Experts.from_linears(plain[:2] + [torch.nn.Linear(8, 4)], [None] * 3)
+    for short in (plain[:2], plain + plain):
+        with pytest.raises(ValueError):
+            int8_utils.Int8Experts.from_linears(short, [None] * 3)
+
+
 CONVERSIONS = [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
                lambda m: m.float(), lambda m: m.bfloat16().float(), lambda m: m.type(torch.float16)]
 
