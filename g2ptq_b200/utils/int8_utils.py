@@ -21,14 +21,20 @@ def _int8_rows(codes):
     return out
 
 
+def _plain_rows(x):
+    """``x [M, K]`` with unit column stride and rows that do not overlap (a broadcast
+    tensor's lie on top of each other)."""
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        return x.contiguous()
+    return x
+
+
 def int8_linear(x, codes, scale, bias=None):
     """``x @ (scale[:, None] * codes).T + bias`` with ``x [..., K]`` quantized per
     token: int8 ``codes [N, K]``, fp32 ``scale [N]`` and ``bias [N]``.  The result
     has ``x``'s type."""
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    if x2.shape[1] > 1 and x2.stride(1) != 1:
-        x2 = x2.contiguous()
-    y = ops.int8_linear(x2, codes, scale, bias)
+    y = ops.int8_linear(_plain_rows(x2), codes, scale, bias)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], y.shape[1])
 
 
@@ -37,9 +43,7 @@ def int8_experts(x, codes, scale, offsets):
     ``offsets[e]`` to ``offsets[e + 1] - 1`` of ``x [R, K]`` through expert
     ``e``'s ``codes [E, N, K]`` and ``scale [E, N]``.  Rows behind the last
     expert's give zeros."""
-    if x.dim() == 2 and x.shape[1] > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    return ops.int8_linear_grouped(x, codes, scale, offsets)
+    return ops.int8_linear_grouped(_plain_rows(x) if x.dim() == 2 else x, codes, scale, offsets)
 
 
 def weight_codes(weight, quantizer):

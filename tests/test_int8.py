@@ -190,6 +190,26 @@ def test_experts_from_what_they_cannot_hold(monkeypatch):
             int8_utils.Int8Experts.from_linears(short, [None] * 3)
 
 
+def test_rows_that_overlap_are_laid_out(monkeypatch):
+    """A broadcast token, or windows over one, reach the product as plain rows."""
+    seen = []
+    monkeypatch.setattr(ops, "int8_linear", lambda x, *a: seen.append(x) or x[:, :1])
+    monkeypatch.setattr(ops, "int8_linear_grouped", lambda x, *a: seen.append(x) or x[:, :1])
+    row = torch.arange(8.0)
+    for x in (row.expand(5, 8), row.expand(2, 3, 8), row.unfold(0, 4, 1), row[::2].expand(3, 4),
+              torch.ones(4, 1).expand(4, 8), row.reshape(8, 1)[:1].expand(6, 1)):
+        int8_utils.int8_linear(x, None, None)
+        if x.dim() == 2:
+            int8_utils.int8_experts(x, None, None, None)
+        for got in seen:
+            assert got.stride(0) >= got.shape[1] and got.stride(1) == 1
+            assert torch.equal(got, x.reshape(-1, x.shape[-1]))
+        seen.clear()
+    plain = torch.ones(5, 16)[:, 4:12]
+    int8_utils.int8_linear(plain, None, None)
+    assert seen[0] is plain  # rows apart are no copy
+
+
 CONVERSIONS = [lambda m: m.to(torch.bfloat16), lambda m: m.half(), lambda m: m.double(),
                lambda m: m.float(), lambda m: m.bfloat16().float(), lambda m: m.type(torch.float16)]
 
@@ -675,6 +695,22 @@ def test_int8_linear_transposed_input():
     codes, scale = aligned_codes((50, 64), g), torch.ones(50, device=DEV)
     q, s = plain_quantize(x)
     check_product(int8_utils.int8_linear(x, codes, scale), q, s, codes, scale, None)
+
+
+@gpu
+def test_int8_linear_broadcast_input():
+    g = gen(5)
+    codes, scale = aligned_codes((50, 64), g), torch.ones(50, device=DEV)
+    off = torch.tensor([0, 7], dtype=torch.int32, device=DEV)
+    row = torch.randn(64, generator=g, device=DEV)
+    for x in (row.expand(7, 64), torch.randn(70, generator=g, device=DEV).unfold(0, 64, 1)):
+        q, s = plain_quantize(x)
+        check_product(int8_utils.int8_linear(x, codes, scale), q, s, codes, scale, None)
+        check_product(int8_utils.int8_experts(x, codes[None], scale[None], off), q, s, codes,
+                      scale, None)
+    y = int8_utils.int8_linear(row.expand(2, 3, 64), codes, scale)
+    q, s = plain_quantize(row.expand(6, 64))
+    check_product(y.reshape(6, 50), q, s, codes, scale, None)
 
 
 @gpu
