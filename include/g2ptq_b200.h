@@ -470,7 +470,8 @@ int g2q_quantize_tokens(int8_t* codes, int64_t ldq, float* scale, const void* x,
  * [N] and bias [N] (may be NULL), out [M, N] of type out_dtype (row stride
  * ldo).  The sums are exact 32-bit integers: K above 131071 is unsupported.
  * Operands whose bases and row strides are multiples of 16 bytes run on the
- * tensor cores, others on the CUDA cores.  `workspace`:
+ * tensor cores, others on the CUDA cores (up to 65535 pieces of 64 rows, more
+ * are unsupported).  `workspace`:
  * g2q_int8_matmul_workspace_bytes(M, N, K) bytes (0 for most shapes). */
 size_t g2q_int8_matmul_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int g2q_int8_matmul(void* out, int out_dtype, int64_t ldo, const int8_t* a, int64_t lda,
