@@ -97,14 +97,19 @@ struct RowScale {
   float scale, below, above;
 };
 
+constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum's low bits are the integer's
+
 // The real quotient's rounding, ties to even, where it lies next to the
-// half-integer between the neighbouring integers a and b: the sign of the exactly
-// rounded residual v - h * scale tells on which side.
-__device__ __forceinline__ int settle(float v, float scale, float a, float b) {
-  const float lo = fminf(a, b), hi = fmaxf(a, b);
-  const float res = fmaf(-(lo + 0.5f), scale, v);
-  const float even = (static_cast<int>(lo) & 1) ? hi : lo;
-  return static_cast<int>(res > 0.f ? hi : (res < 0.f ? lo : even));
+// half-integer between the neighbouring integers of a and b (sums with kMagic, like
+// the result): the sign of the exactly rounded residual v - h * scale tells on
+// which side.  Of the smallest scales twice that: it is a multiple of 2^-150, which
+// alone would round to zero.
+__device__ __forceinline__ uint32_t settle(float v, float scale, float a, float b) {
+  const float lo = fminf(a, b), hi = fmaxf(a, b), n = lo - kMagic;
+  float res = fmaf(-(n + 0.5f), scale, v);
+  if (scale < 1e-36f) res = fmaf(-(n + n + 1.f), scale, v + v);
+  const float even = (__float_as_uint(lo) & 1) ? hi : lo;
+  return __float_as_uint(res > 0.f ? hi : (res < 0.f ? lo : even));
 }
 
 // Codes of a unit, four to a word: round(v / scale) of the real quotient.  Where
@@ -114,7 +119,6 @@ __device__ __forceinline__ int settle(float v, float scale, float a, float b) {
 // scale's own rounding.
 template <typename S>
 __device__ __forceinline__ void unit_codes(const Unit<S>& u, const RowScale& rs, uint32_t (&w)[4]) {
-  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23: a sum's low byte is the integer's
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
     uint32_t a[4], b[4];
@@ -135,10 +139,9 @@ __device__ __forceinline__ void unit_codes(const Unit<S>& u, const RowScale& rs,
       const float v01 = i & 1 ? u.at(4 * g + 1) : u.at(4 * g);
       const float v23 = i & 1 ? u.at(4 * g + 3) : u.at(4 * g + 2);
       const float v = i & 2 ? v23 : v01;
-      const int code = settle(v, rs.scale, fmaf(v, rs.below, kMagic) - kMagic,
-                              fmaf(v, rs.above, kMagic) - kMagic);
+      const uint32_t code = settle(v, rs.scale, fmaf(v, rs.below, kMagic), fmaf(v, rs.above, kMagic));
       const uint32_t mask = 255u << (8 * i);
-      w[g] = (w[g] & ~mask) | ((static_cast<uint32_t>(code) << (8 * i)) & mask);
+      w[g] = (w[g] & ~mask) | ((code << (8 * i)) & mask);
       differ &= ~mask;
     }
   }

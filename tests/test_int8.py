@@ -329,6 +329,34 @@ def test_quantize_near_ties():
 
 
 @gpu
+def test_quantize_near_ties_of_the_smallest_scales():
+    """Quotients half a unit of the smallest fp32 number beside a half-integer: their
+    distance from it, 2^-150, is no fp32 number itself."""
+    unit = 2.0 ** -149
+    steps = torch.arange(200, dtype=torch.int64)
+    top = (127 * (2 ** 23 + 1000 + 9973 * steps)).double() * unit  # scales from 2^-126 up
+    scale = (top.float().double() / 127).float()
+    size = (scale.double() / unit).long()  # in units
+    odd = size % 2 == 1
+    assert int(odd.sum()) > 50 and bool((size[odd] < 2 ** 24 * 2 // 3).all())
+    size, top = size[odd], top[odd].float()
+    v = torch.stack([(size + 1) // 2, (size - 1) // 2, (3 * size + 1) // 2, (3 * size - 1) // 2], 1)
+    x = torch.cat([top[:, None], (v.double() * unit).float(), (-v.double() * unit).float()], 1)
+    # by whole numbers: round(v / size) lies where 2 v does beside the odd multiples of size
+    want = torch.tensor([[127, 1, 0, 2, 1, -1, 0, -2, -1]]).expand(len(x), 9).to(torch.int8)
+    q, s = plain_quantize(x)
+    assert torch.equal(q, want)
+    for rep in (1, 400 // len(x) + 1):  # few rows and many
+        got, gs = ops.quantize_tokens(x.to(DEV).repeat(rep, 1))
+        assert torch.equal(gs.cpu(), s.repeat(rep))
+        assert torch.equal(got.cpu(), want.repeat(rep, 1))
+    one = ops.int8_linear(x[:1].to(DEV), torch.eye(9, dtype=torch.int8, device=DEV),
+                          torch.full((9,), 2.0 ** 126, device=DEV))  # in the product's own kernel
+    assert torch.equal(torch.round(one.cpu().double() / (s[0].double() * 2.0 ** 126)),
+                       want[:1].double())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("C", [24, 1500, 20000])
 def test_quantize_odd_rows(dtype, C):
