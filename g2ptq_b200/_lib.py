@@ -175,7 +175,8 @@ def binding():
     import torch  # noqa: F401  (its libraries have to be loaded first)
     from . import ops
     lib = load()
-    spec = importlib.util.spec_from_file_location("_binding", path)
+    # by its full name: modules of one name are one module to pybind11
+    spec = importlib.util.spec_from_file_location(__package__ + "._binding", path)
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     mod.bind({n: ctypes.cast(getattr(lib, n), P).value for n in _BOUND}, G2QError,

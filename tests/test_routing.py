@@ -333,6 +333,20 @@ def test_forward_mode_is_refused():
                 call()
 
 
+def test_another_extension_of_the_same_short_name(tmp_path):
+    """Some other package's extension called _binding is not this one."""
+    import importlib.util
+    import shutil
+    from g2ptq_b200 import build
+    mine = _lib.binding()
+    path = str(tmp_path / "_binding.so")
+    shutil.copy(build.BINDING, path)
+    spec = importlib.util.spec_from_file_location("_binding", path)
+    other = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(other)
+    assert other is not mine and mine.__spec__.origin == build.BINDING
+
+
 @gpu
 def test_a_refused_size_is_a_library_error():
     # more elements per slot than the library indexes: refused before any launch
