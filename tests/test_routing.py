@@ -360,6 +360,76 @@ def test_a_refused_size_is_a_library_error():
                   8, None)
 
 
+def failing_binding(tmp_path, names, status):
+    """A second copy of the binding, in which the library's functions `names` return
+    `status` without doing anything."""
+    import importlib.util
+    import shutil
+    from g2ptq_b200 import build
+    path = str(tmp_path / "_binding.so")
+    shutil.copy(build.BINDING, path)
+    _lib.binding()  # torch and the library are loaded
+    failing_binding.keep.append(path)
+    spec = importlib.util.spec_from_file_location(
+        f"failing{len(failing_binding.keep)}._binding", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    fail = ctypes.CFUNCTYPE(ctypes.c_int)(lambda: status)
+    failing_binding.keep.append(fail)  # called by address, so never freed
+    address = {n: ctypes.cast(getattr(_lib.load(), n), ctypes.c_void_p).value for n in _lib._BOUND}
+    address.update({n: ctypes.cast(fail, ctypes.c_void_p).value for n in names})
+    mod.bind(address, _lib.G2QError, lambda idx: 0)
+    return mod
+
+
+failing_binding.keep = []
+
+
+@gpu
+def test_errors_of_the_library_reach_the_caller(tmp_path):
+    g = gen(6)
+    ids = torch.randint(0, 4, (9, 2), generator=g, device=DEV)
+    r = moe_utils.route(ids, 4)
+    x, y = (torch.randn(n, 8, generator=g, device=DEV) for n in (9, 18))
+    w = torch.rand(9, 2, generator=g, device=DEV)
+    names = ("g2q_route", "g2q_dispatch_rows", "g2q_combine_rows", "g2q_combine_rows_backward")
+    mod = failing_binding(tmp_path, names, _lib.G2Q_ERR_UNSUPPORTED)
+    for name, call in zip(names, (
+            lambda m: m.route(ids, 4), lambda m: m.dispatch_rows(x, r.position),
+            lambda m: m.combine_rows(y, r.position, w),
+            lambda m: m.combine_rows_backward(x, y, r.position, w, True, True))):
+        with pytest.raises(_lib.G2QError, match=f"{name}.*unsupported") as e:
+            call(mod)
+        assert e.value.status == _lib.G2Q_ERR_UNSUPPORTED
+        call(_lib.binding())
+    for call in (lambda m: m.dispatch(x.clone().requires_grad_(), r.position),
+                 lambda m: m.combine(y.clone().requires_grad_(), r.position, w)):
+        with pytest.raises(_lib.G2QError):
+            call(mod)
+        assert call(_lib.binding()).requires_grad
+
+
+@gpu
+def test_errors_of_the_library_in_a_backward(tmp_path):
+    """There the engine's thread has no interpreter to make a G2QError with: a plain
+    error of the same text, and the process goes on."""
+    g = gen(7)
+    r = moe_utils.route(torch.randint(0, 4, (9, 2), generator=g, device=DEV), 4)
+    y = torch.randn(18, 8, generator=g, device=DEV).requires_grad_()
+    w = torch.rand(9, 2, generator=g, device=DEV).requires_grad_()
+    mod = failing_binding(tmp_path, ("g2q_combine_rows_backward", "g2q_dispatch_rows"),
+                          _lib.G2Q_ERR_INVALID_ARG)
+    with pytest.raises(RuntimeError, match="g2q_combine_rows_backward failed: .*invalid argument"):
+        mod.combine(y, r.position, w).sum().backward()
+    with pytest.raises(RuntimeError, match="g2q_dispatch_rows failed: .*invalid argument"):
+        mod.combine(y, r.position, None).sum().backward()
+    assert y.grad is None and w.grad is None
+    moe_utils.combine(y, r, w).sum().backward()
+    gy, gw = ops.combine_rows_backward(torch.ones(9, 8, device=DEV), y.detach(), r.position,
+                                       w.detach())
+    assert torch.equal(y.grad, gy) and torch.equal(w.grad, gw)
+
+
 @gpu
 def test_second_derivatives_are_refused():
     g = gen(4)
