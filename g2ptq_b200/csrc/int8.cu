@@ -348,7 +348,7 @@ extern "C" int g2q_int8_linear(void* out, int out_dtype, int64_t ldo, const void
   if (!x || (need && (!workspace || !rows::aligned(workspace, 16) || workspace_bytes < need)))
     return G2Q_ERR_INVALID_ARG;
   if (i8::stream_quantizes(p))
-    return i8::stream_linear(p, x, x_dtype, ldx, (cudaStream_t)stream);
+    return i8::stream_linear(p, x, x_dtype, (cudaStream_t)stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const size_t code_bytes = i8::up256((size_t)M * (size_t)ld);
   const size_t scale_bytes = i8::up256((size_t)M * sizeof(float));

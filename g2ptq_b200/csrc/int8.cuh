@@ -109,12 +109,12 @@ int tc_product(const Product& p, void* workspace, size_t workspace_bytes, bool o
                cudaStream_t st);
 
 // The product for a handful of tokens (int8_stream.cu): whether it takes these
-// operands (aligned like above), the launch, and the same with the tokens
+// operands (aligned like above), the launch, and the same with a single token
 // quantized by the kernel itself.
 bool stream_takes(const Product& p);
 int stream_product(const Product& p, bool overlap, cudaStream_t st);
 bool stream_quantizes(const Product& p);
-int stream_linear(const Product& p, const void* x, int x_dtype, long long ldx, cudaStream_t st);
+int stream_linear(const Product& p, const void* x, int x_dtype, cudaStream_t st);
 
 }  // namespace i8
 }  // namespace g2q

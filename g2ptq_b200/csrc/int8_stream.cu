@@ -109,20 +109,24 @@ __device__ __forceinline__ bool find_group(const Product& p, int slot, int* grou
   return false;
 }
 
-struct Input {  // the tokens before quantization (FUSED)
+struct Input {  // the token before quantization (FUSED)
   const void* x;
-  long long ldx;
   bool vec;
 };
 
-// MG groups of eight tokens at a time.
+// Bytes of one token's codes in shared memory, zeros behind the last column.
+__host__ __device__ __forceinline__ int fused_bytes(const Product& p) {
+  return (int)((p.K + 127) / 128 * 128);
+}
+
+// MG groups of eight tokens at a time; FUSED: one token.
 template <typename S, typename X, int RG, int MG, bool FUSED>
 __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const Input in) {
   constexpr int KS = SW / RG, TOKENS = 8 * MG, CHANNELS = 16 * RG;
   // steps whose loads are in flight together (eight instead of four: 5.3 -> 5.0 us
   // for eight tokens through 4096 x 4096; with more channels per CTA slower)
   constexpr int DEPTH = RG == 1 && MG == 1 ? 8 : 4;
-  extern __shared__ uint4 dyn[];  // FUSED: codes [M][pitch]
+  extern __shared__ uint4 dyn[];  // FUSED: the token's codes
   __shared__ int red[KS][CHANNELS][TOKENS + 1];
   __shared__ float sa_s[TOKENS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -162,14 +166,11 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
   load_w(ks);
   tc::wait_predecessor();  // the tokens' codes and scales; the weight does not depend on them
 
-  const int pitch = (int)((p.K + 127) / 128 * 128) + 64;
   int8_t* codes = reinterpret_cast<int8_t*>(dyn);
   if (FUSED) {
-    const X* x = static_cast<const X*>(in.x);
     __shared__ unsigned tops[SW];
-    for (int m = 0; m < (int)p.M; ++m)
-      quantize_row<X, 32 * SW>(codes + (long long)m * pitch, pitch - 64, &sa_s[m],
-                               x + m * in.ldx, (int)p.K, in.vec, tops);
+    quantize_row<X, 32 * SW>(codes, fused_bytes(p), sa_s, static_cast<const X*>(in.x), (int)p.K,
+                             in.vec, tops);
     __syncthreads();
   }
 
@@ -193,7 +194,7 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
           const int m = 8 * j + g;
           tok[d][j] = make_uint4(0, 0, 0, 0);
           if (m < have && k < p.K) {
-            if (FUSED) tok[d][j] = *reinterpret_cast<const uint4*>(codes + (long long)m * pitch + k);
+            if (FUSED) tok[d][j] = *reinterpret_cast<const uint4*>(codes + k);
             else tok[d][j] = load16<false>(p.a + (m0 + m) * p.lda, k, p.K);
           }
         }
@@ -238,12 +239,11 @@ __global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const 
 // tokens of 4096 columns 8.2 and 5.3 us.
 constexpr long long kFusedColumns = 8192;
 
-static long long fused_bytes(const Product& p) { return p.M * ((p.K + 127) / 128 * 128 + 64); }
-
 bool stream_takes(const Product& p) {
   if (!tc_takes(p)) return false;  // the same alignment
-  // one group: two groups of eight tokens; groups: few rows each on average, so
-  // that hardly any weight is read more than once
+  // one group: two groups of eight tokens; groups: few rows each on average, whose
+  // weights are then read once as long as the rows are spread evenly (a group of
+  // many rows reads its weight again for every eight of them)
   if (p.offsets) return p.M <= 2 * p.groups && p.M <= 4096;
   // more than eight tokens double the work per weight byte: 14336 channels x 4096
   // took 20.6 us here and 17.1 us on the tiles, 4096 x 4096 6.4 and 11.5 us
@@ -260,7 +260,7 @@ static int launch_stream(const Product& p, const Input& in, bool overlap, cudaSt
   cfg.gridDim = dim3((unsigned)cdiv(p.N, 16 * RG), 
                      p.offsets ? (unsigned)(p.groups < p.M ? p.groups + 1 : p.M) : 1, 1);
   cfg.blockDim = dim3(32 * SW, 1, 1);
-  cfg.dynamicSmemBytes = FUSED ? (size_t)fused_bytes(p) : 0;
+  cfg.dynamicSmemBytes = FUSED ? fused_bytes(p) : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -278,7 +278,7 @@ static int launch_stream(const Product& p, const Input& in, bool overlap, cudaSt
 
 template <typename S>
 static int stream_out(const Product& p, bool overlap, cudaStream_t st) {
-  const Input none = {nullptr, 0, false};
+  const Input none = {nullptr, false};
   if (p.offsets) return launch_stream<S, float, 4, 1, false>(p, none, overlap, st);
   // every warp needs a turn of K (512 bytes of it for eight tokens and one channel
   // group per CTA, else 256): 14336 channels x 1024 took 11.1 us with eight warps
@@ -315,10 +315,8 @@ static int stream_in(const Product& p, const Input& in, cudaStream_t st) {
   return stream_in_out<float, X>(p, in, st);
 }
 
-int stream_linear(const Product& p, const void* x, int x_dtype, long long ldx, cudaStream_t st) {
-  const Input in = {x, ldx,
-                    rows::aligned(x, 16) &&
-                        (p.M <= 1 || ldx * rows::elem_bytes(x_dtype) % 16 == 0)};
+int stream_linear(const Product& p, const void* x, int x_dtype, cudaStream_t st) {
+  const Input in = {x, rows::aligned(x, 16)};
   if (x_dtype == G2Q_DTYPE_BF16) return stream_in<__nv_bfloat16>(p, in, st);
   if (x_dtype == G2Q_DTYPE_F16) return stream_in<__half>(p, in, st);
   return stream_in<float>(p, in, st);

@@ -154,8 +154,7 @@ __global__ void __launch_bounds__(SORT_THREADS) route_place_kernel(SortArgs a) {
         part[w * E1 + e] = (uint16_t)run;
         run += c;
       }
-      if (ONE) total[e] = run;
-      else total[e] = run;  // of this chunk, from here on
+      total[e] = run;  // of this chunk, from here on
     }
     __syncthreads();
     if (ONE) {
