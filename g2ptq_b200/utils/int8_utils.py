@@ -24,9 +24,10 @@ def _int8_rows(codes):
 def _plain_rows(x):
     """``x [M, K]`` with unit column stride and rows that do not overlap (a broadcast
     tensor's lie on top of each other)."""
-    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
-        return x.contiguous()
-    return x
+    if x.is_contiguous():
+        return x
+    (rows, cols), (step, unit) = x.shape, x.stride()
+    return x.contiguous() if (cols > 1 and unit != 1) or (rows > 1 and step < cols) else x
 
 
 def int8_linear(x, codes, scale, bias=None):
