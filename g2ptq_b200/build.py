@@ -51,7 +51,12 @@ def build_binding(verbose=False):
 def build(jobs=None, verbose=False):
     jobs = jobs or max(1, min(16, os.cpu_count() or 1))
     _run(["make", "-C", os.path.join(HERE, "csrc"), f"-j{jobs}"], "libg2ptq_b200.so", verbose)
-    build_binding(verbose)
+    try:
+        build_binding(verbose)
+    except (RuntimeError, OSError) as e:
+        raise RuntimeError("libg2ptq_b200.so is built and runs the quantization path; its torch "
+                           "binding, which the 8-bit linears and the expert routing need, is not "
+                           f"(g++ and the headers of Python and torch): {e}") from e
     return os.path.join(HERE, "_lib", "libg2ptq_b200.so")
 
 

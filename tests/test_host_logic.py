@@ -382,3 +382,21 @@ def test_weight_quantizer_deepcopy_is_independent():
     assert float(q.scale) == 0.0 and float(qs[1].scale) == 0.0
     c = copy.deepcopy(qs[0])
     assert float(c.scale) == 5.0 and c.scale is not qs[0].scale
+
+
+def test_a_failing_binding_leaves_the_library(monkeypatch):
+    """Without the headers of Python or torch the build says what is there and what is
+    not."""
+    from g2ptq_b200 import build
+    ran = []
+
+    def run(cmd, what, verbose):
+        ran.append(what)
+        if "binding" in what:
+            raise RuntimeError(f"building {what} failed")
+
+    monkeypatch.setattr(build, "_run", run)
+    monkeypatch.setattr(build, "BINDING", build.BINDING + ".none")
+    with pytest.raises(RuntimeError, match="is built and runs the quantization path.*binding"):
+        build.build()
+    assert ran == ["libg2ptq_b200.so", "the torch binding"]
