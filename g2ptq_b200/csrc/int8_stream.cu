@@ -119,9 +119,18 @@ __host__ __device__ __forceinline__ int fused_bytes(const Product& p) {
   return (int)((p.K + 127) / 128 * 128);
 }
 
+// CTAs per SM: two of the variants with the most loads in flight, else three, four
+// where a 16-bit token is quantized (64 registers: 448 CTAs of 14336 channels x 4096
+// are one wave, 13.8 us; 72 registers took 16.6).
+template <typename X, int RG, int MG, bool FUSED>
+constexpr int stream_ctas() {
+  return RG == 1 || MG == 2 ? 2 : (FUSED && sizeof(X) == 2 ? 4 : 3);
+}
+
 // MG groups of eight tokens at a time; FUSED: one token.
 template <typename S, typename X, int RG, int MG, bool FUSED>
-__global__ void __launch_bounds__(32 * SW) stream_kernel(const Product p, const Input in) {
+__global__ void __launch_bounds__(32 * SW, stream_ctas<X, RG, MG, FUSED>())
+    stream_kernel(const Product p, const Input in) {
   constexpr int KS = SW / RG, TOKENS = 8 * MG, CHANNELS = 16 * RG;
   // steps whose loads are in flight together (eight instead of four: 5.3 -> 5.0 us
   // for eight tokens through 4096 x 4096; with more channels per CTA slower)
