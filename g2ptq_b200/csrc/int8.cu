@@ -22,7 +22,7 @@ using rows::of_f;
 
 // G threads per row, UNITS units of 16 elements per thread kept in registers
 // between the maximum and the codes (one read of x): 16384 x 4096 bf16 in 38 us
-// (5.2 TB/s), about even between HBM and issue slots (55 % of each).  What is left of a row --
+// (5.3 TB/s), about even between HBM and issue slots (55 % of each).  What is left of a row --
 // the units beyond UNITS * G, a part of a unit at its end -- goes element by
 // element and is read a second time.  VEC: rows on 16-byte boundaries.
 template <typename S, int G, int UNITS, bool VEC>

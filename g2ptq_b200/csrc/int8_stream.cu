@@ -10,9 +10,10 @@
 // operands use the same, so 16 consecutive bytes serve as the four words that a
 // lane owes two steps.  The warps' integer sums meet in shared memory.
 //
-// Measured: one token through 4096 x 4096 in 4.6 us, 14336 x 4096 in 13.0 us (4.5
-// TB/s), eight tokens through 14336 x 16384 in 48 us (4.9 TB/s; a plain sum of as
-// many bytes reads 5.3): bound by reading the weight.
+// Measured: one token through 4096 x 4096 in 4.5 us with the weight in L2 and 6.0 us
+// from memory, 14336 x 4096 in 13.8 us (4.3 TB/s), eight tokens through 14336 x
+// 16384 in 48 us (4.9 TB/s; a plain sum of as many bytes reads 5.3): bound by
+// reading the weight.
 //
 // A single token's codes are made by the kernel itself (FUSED): every CTA makes
 // them in shared memory, behind its first weight loads.

@@ -22,7 +22,7 @@
 // Gram kernels; on expiry G2Q_ERR_TIMEOUT goes to the status word and the CTAs
 // wind down.
 //
-// Measured: 16384 x 14336 x 4096 in 596-615 us (3.2 POP/s, tensor pipe 88.6 %
+// Measured: 16384 x 14336 x 4096 in 596-615 us (3.2 POP/s, tensor pipe 88.4 %
 // active; 730-770 us once the card is at its power limit), bound by the pipe;
 // 65536 rows of 768 through 128 experts of 2048 channels in 123-129 us, bound by
 // the epilogue (6.2k cycles per tile, of which the MMAs need 3.05k); 24 tokens
