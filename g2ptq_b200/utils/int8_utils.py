@@ -121,7 +121,8 @@ class Int8Experts(_Int8Weight):
     def from_linears(cls, linears, quantizers):
         """One quantizer per linear.  Linears with a bias are refused: the grouped
         product has none."""
-        if any(lin.bias is not None for lin in linears):
+        linears = list(linears)
+        if any(getattr(lin, "bias", None) is not None for lin in linears):
             raise ValueError("8-bit experts have no bias; a linear that has one needs Int8Linear")
         pairs = [weight_codes(lin.weight.data, q)
                  for lin, q in zip(linears, quantizers, strict=True)]

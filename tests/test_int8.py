@@ -183,6 +183,8 @@ def test_experts_from_what_they_cannot_hold(monkeypatch):
                         lambda w, q: (torch.zeros(w.shape, dtype=torch.int8), torch.ones(len(w))))
     plain = [torch.nn.Linear(8, 4, bias=False) for _ in range(3)]
     assert int8_utils.Int8Experts.from_linears(plain, [None] * 3).codes.shape == (3, 4, 8)
+    m = int8_utils.Int8Experts.from_linears((lin for lin in plain), iter([None] * 3))
+    assert m.codes.shape == (3, 4, 8)
     with pytest.raises(ValueError, match="bias"):
         int8_utils.Int8Experts.from_linears(plain[:2] + [torch.nn.Linear(8, 4)], [None] * 3)
     for short in (plain[:2], plain + plain):
